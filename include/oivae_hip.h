@@ -258,6 +258,87 @@ int oivae_adam_f32(float* p, const float* g, float* m, float* v, int64_t n,
                    float lr, float beta1, float beta2, float eps, int32_t step,
                    float grad_scale, void* stream);
 
+/* ---- AdamW, gradient norm and clipping over lists of tensors -----------------------------------------------------
+ * No counterpart in the reference, whose scripts step their modules with torch.optim.Adam one tensor at a time
+ * (data_vs_test_loss_autoencoder.py:96-145).  torch.optim.AdamW's update (decoupled weight decay), with the clipping of
+ * torch.nn.utils.clip_grad_norm_ in front of it:
+ *   norm = |grad_scale| * sqrt(sum over all tensors of g^2)          (squares and sums in fp64, in a fixed order)
+ *   coef = min(1, max_norm / (norm + 1e-6)); 1 when max_norm <= 0
+ *   g~ = g * grad_scale * coef;  m = b1 m + (1-b1) g~;  v = b2 v + (1-b2) g~^2
+ *   w = w (1 - lr wd) - lr/(1-b1^t) * m / (sqrt(v)/sqrt(1-b2^t) + eps)
+ * The tensor lists are HOST arrays, read during the call; nothing is uploaded and no pointer is kept.
+ * A tensor is dense memory of n elements (any alignment that its element type allows); gradient and parameter share the
+ * order of their elements.  Parameters of 16 bits are rounded copies (to nearest) of fp32 master weights. */
+enum { OIVAE_F32 = 0, OIVAE_BF16 = 1, OIVAE_F16 = 2 };
+#define OIVAE_ADAMW_BLOCK 128   /* a tensor's place in the moment buffers is a whole number of these blocks */
+
+typedef struct {
+  void* g;          /* device */
+  int64_t n;
+  int32_t type;     /* OIVAE_F32 | OIVAE_BF16 | OIVAE_F16 */
+  int32_t pad;
+} oivae_grad_t;
+
+/* Verdict of oivae_grad_norm, on the device; zero it once before its first use. */
+typedef struct {
+  float norm, coef;
+  int32_t skip;      /* 1: the norm is not finite (or a decoder launch behind the gradients failed): oivae_adamw_* leave
+                        everything untouched */
+  int32_t skipped;   /* steps left out so far (counted where step counters are given) */
+} oivae_clip_t;
+
+typedef struct {
+  void* p;           /* parameter (device) */
+  const void* g;     /* gradient (device) */
+  int64_t n;
+  int64_t at;        /* first element in the moment (and master) buffers: a multiple of OIVAE_ADAMW_BLOCK; the tensor owns
+                        [at, at + n rounded up to whole blocks), which start at zero */
+  int32_t p_type, g_type;
+  int32_t group;     /* index into the groups */
+  int32_t index;     /* of its step counter; distinguishes its random bits (oivae_adamw_f8) */
+  int32_t step;      /* t >= 1, the step being taken; not read where the state holds step counters */
+  int32_t pad;
+} oivae_adamw_tensor_t;
+
+typedef struct {
+  float lr, weight_decay;
+  const float* lr_dev;   /* one float on the device, read instead of lr when not NULL (a captured graph's schedule) */
+} oivae_adamw_group_t;
+
+/* Flat buffers on the device, 16-byte aligned.  oivae_adamw_f32: m, v floats; the scales are not read.
+ * oivae_adamw_f8: m e4m3 codes, v e5m2 codes (OCP formats), m_scale / v_scale one e8m0 byte per block of 128 elements:
+ * a code's value times 2^(byte - 127); byte 255 (a NaN or an infinity reached the block) makes the block NaN. */
+typedef struct {
+  void* m;
+  void* v;
+  uint8_t* m_scale;
+  uint8_t* v_scale;
+  float* master;         /* fp32 weights of the 16-bit parameters; may be NULL when there are none */
+  const int32_t* steps;  /* step counters by tensor index, as oivae_grad_norm left them; NULL: the tensors' own `step` */
+} oivae_adamw_state_t;
+
+/* Norm, coefficient and verdict into `clip`; then, unless the step is to be left out, steps[which[i]] += 1 for the
+ * n_which counters named (host array; steps may be NULL with n_which = 0).  count = 0 gives norm 0.
+ * workspace: oivae_grad_norm_workspace_bytes(count) bytes on the device, 8-byte aligned. */
+int64_t oivae_grad_norm_workspace_bytes(int32_t count);
+int oivae_grad_norm(const oivae_grad_t* grads, int32_t count, float grad_scale, float max_norm, oivae_clip_t* clip,
+                    int32_t* steps, const int32_t* which, int32_t n_which, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
+/* g *= clip->coef in place (nothing is touched when it is 1). */
+int oivae_grad_clip(const oivae_grad_t* grads, int32_t count, const oivae_clip_t* clip, void* stream);
+
+/* One AdamW step of `count` tensors; `clip` (may be NULL) from oivae_grad_norm on the same stream. */
+int oivae_adamw_f32(const oivae_adamw_tensor_t* tensors, int32_t count, const oivae_adamw_group_t* groups, int32_t n_groups,
+                    const oivae_adamw_state_t* state, double beta1, double beta2, double eps, float grad_scale,
+                    const oivae_clip_t* clip, void* stream);
+
+/* The same with moments of 8 bits, rounded stochastically: the random bits are a function of (seed, t, tensor index,
+ * element index), so a step repeated from the same state gives the same bits. */
+int oivae_adamw_f8(const oivae_adamw_tensor_t* tensors, int32_t count, const oivae_adamw_group_t* groups, int32_t n_groups,
+                   const oivae_adamw_state_t* state, double beta1, double beta2, double eps, float grad_scale,
+                   uint32_t seed, const oivae_clip_t* clip, void* stream);
+
 /* ---- the whole step of a small model in one launch ------------------------------------------------------------
  * Replaces OIVAE.step (lib/oivae.py:42-90) in one call for the shapes the reference's own scripts train
  * (bars_data_oivae.py:20-33, mo_mo_mocap_oivae.py:26-35): encoder forward + KL + samples, grouped decoder forward /

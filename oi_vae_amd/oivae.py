@@ -5,7 +5,7 @@ import torch
 from . import _lib, parallel
 from .adopt import adopt, probe_encoder_head
 from .distributions import Normal
-from .optim import SGD as _EngineSGD, _EngineOptimizer
+from .optim import Adam as _EngineAdam, SGD as _EngineSGD, _EngineOptimizer
 
 
 class NormalPriorTheta(object):
@@ -58,8 +58,8 @@ class OIVAE(object):
         opt._attach(self.engine)
         if isinstance(opt, _EngineSGD):
           self._fused_sgd = opt
-        else:
-          self._fused_adam = opt
+        elif isinstance(opt, _EngineAdam):
+          self._fused_adam = opt   # (AdamW steps the flat buffers by itself, after every gradient is final)
       else:
         ps = [p for g in opt.param_groups for p in g["params"]]
         self._foreign.append((opt, [(p, grad_of[id(p)]) for p in ps if id(p) in grad_of]))

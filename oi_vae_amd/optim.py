@@ -6,8 +6,17 @@ engine (after `OIVAE(...)` adopted the model) they update them with ONE fused
 HIP kernel each over the engine's flat buffers instead of one launch per
 tensor; `SGD` on `Ws` is fused with the proximal step that follows it.
 torch.optim optimizers keep working too (the parameters are ordinary views).
+
+`AdamW` also steps parameters that no engine holds (torch modules on the GPU, such as the
+autoencoder variant's), all of them in a few launches, with moments in 32 or in 8 bits;
+`clip_grad_norm_` and `grad_norm` are the gradient norm over such parameters.
 """
+import ctypes
+
+import numpy as np
 import torch
+
+from . import _lib
 
 
 class _EngineOptimizer(object):
@@ -90,3 +99,393 @@ class SGD(_EngineOptimizer):
     if self.fused_with_prox:
       return  # OIVAE.step runs oivae_sgd_prox_f32 right after the optimizers
     self._engine.sgd_prox_step(self._lr(), 0.0, do_prox=False)
+
+
+# ---- lists of tensors ------------------------------------------------------------------------------------------------------
+_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_GRAD = np.dtype([("g", "u8"), ("n", "i8"), ("type", "i4"), ("pad", "i4")])                       # oivae_grad_t
+_TENSOR = np.dtype([("p", "u8"), ("g", "u8"), ("n", "i8"), ("at", "i8"), ("p_type", "i4"), ("g_type", "i4"),
+                    ("group", "i4"), ("index", "i4"), ("step", "i4"), ("pad", "i4")])             # oivae_adamw_tensor_t
+_GROUP = np.dtype([("lr", "f4"), ("weight_decay", "f4"), ("lr_dev", "u8")])                       # oivae_adamw_group_t
+
+
+def _dense(t):
+  """Whether t's elements fill one piece of memory, in any order of its dimensions."""
+  if t.layout != torch.strided:
+    return False
+  expect = 1
+  for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+    if stride != expect:
+      return False
+    expect *= size
+  return True
+
+
+def _check_types(tensors, what):
+  device = None
+  for t in tensors:
+    if not torch.is_tensor(t) or t.layout != torch.strided:
+      raise ValueError("%s must be dense tensors, got %s" % (what, getattr(t, "layout", type(t).__name__)))
+    if t.dtype not in _TYPES:
+      raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (what, t.dtype))
+    if not t.is_cuda:
+      raise _lib.OivaeError("%s must be on the GPU, got %s: there is no CPU fallback" % (what, t.device))
+    if device is not None and t.device != device:
+      raise ValueError("%s must be on one device, got %s and %s" % (what, device, t.device))
+    device = t.device
+  return device
+
+
+def _grads_of(parameters):
+  ps = [parameters] if torch.is_tensor(parameters) else list(parameters)
+  grads = [p.grad for p in ps if p.grad is not None]
+  device = _check_types(grads, "gradients")
+  if len({g.data_ptr() for g in grads if g.numel()}) != sum(1 for g in grads if g.numel()):
+    raise ValueError("the same gradient appears more than once")
+  return grads, device
+
+
+def _norm_of(grads, device, max_norm):
+  L = _lib.init_device(device.index)
+  rec = np.zeros(len(grads), _GRAD)
+  rec["g"] = [g.data_ptr() for g in grads]
+  rec["n"] = [g.numel() for g in grads]
+  rec["type"] = [_TYPES[g.dtype] for g in grads]
+  clip = torch.zeros(4, dtype=torch.float32, device=device)
+  nbytes = L.oivae_grad_norm_workspace_bytes(len(grads))
+  ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+  stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+  _lib.check(L.oivae_grad_norm(rec.ctypes.data, len(grads), 1.0, max_norm, clip.data_ptr(), None, None, 0, ws.data_ptr(), nbytes,
+                               stream), "oivae_grad_norm")
+  return L, rec, clip, stream
+
+
+def grad_norm(parameters):
+  """2-norm of the gradients of `parameters` (a tensor or an iterable of tensors; those without a gradient are left out)
+  taken as one vector: a 0-dim float32 tensor on their device, with no synchronisation.  Squares and sums are formed in
+  fp64, in an order that depends on the sizes alone."""
+  grads, device = _grads_of(parameters)
+  if not grads:
+    return torch.zeros(())
+  with torch.cuda.device(device):
+    return _norm_of([g if _dense(g) else g.contiguous() for g in grads], device, 0.0)[2][0]
+
+
+def clip_grad_norm_(parameters, max_norm):
+  """torch.nn.utils.clip_grad_norm_ (2-norm): scales the gradients in place by min(1, max_norm / (norm + 1e-6)) and returns
+  the norm they had, without synchronising.  A norm that is not finite reaches the gradients as it does there (NaN)."""
+  max_norm = float(max_norm)
+  if not max_norm > 0:
+    raise ValueError("max_norm must be positive, got %r" % max_norm)
+  grads, device = _grads_of(parameters)
+  if not grads:
+    return torch.zeros(())
+  with torch.cuda.device(device):
+    packed = [g if _dense(g) else g.contiguous() for g in grads]
+    L, rec, clip, stream = _norm_of(packed, device, max_norm)
+    _lib.check(L.oivae_grad_clip(rec.ctypes.data, len(packed), clip.data_ptr(), stream), "oivae_grad_clip")
+    for g, c in zip(grads, packed):
+      if c is not g:
+        g.copy_(c)
+    return clip[0]
+
+
+class AdamW(_EngineOptimizer):
+  """torch.optim.AdamW (decoupled weight decay) over many tensors at once.
+
+  Two uses: handed to `OIVAE(optimizers=[AdamW(...), SGD(...)])` it steps the engine's flat buffers in place of `Adam` (one
+  lr, weight_decay and state_bits for all groups); by itself it steps the `.grad` of any float32, bfloat16 or float16
+  tensors on one GPU.  Per group: `lr`, `weight_decay`, `state_bits`; `betas` and `eps` are one for all.
+
+  state_bits=8 holds both moments in 8 bits: blocks of 128 elements of a tensor share a power of two; first moments are
+  e4m3 codes, second moments e5m2 codes, rounded stochastically with bits drawn from (seed, step, tensor, element) -- two
+  runs of one program agree bit for bit.  16-bit parameters are rounded copies of fp32 master weights, which the optimizer
+  keeps; whoever writes such parameters behind its back calls `sync_master()`.
+
+  max_grad_norm: clips by the norm of all gradients of this optimizer (`grad_norm` holds it after a step).  The gradients
+  themselves stay as they are, and a step whose norm is not finite is left out on the device (`skipped` counts them).
+  capturable: keeps the step counts on the device, so that a step captured into a graph advances them (max_grad_norm
+  implies it); `lr` may then be a one-element float32 tensor on the device, which replays read anew.  Touch `buffers` (or
+  take a step) before capturing.  Nothing here synchronises."""
+
+  def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None,
+               capturable=False, seed=0):
+    super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits)
+    if max_grad_norm is not None and not max_grad_norm > 0:
+      raise ValueError("max_grad_norm must be positive or None, got %r" % (max_grad_norm,))
+    if not 0 <= int(seed) < 1 << 32:
+      raise ValueError("seed must be in [0, 2^32), got %r" % (seed,))
+    seen = set()
+    for g in self.param_groups:
+      if g["state_bits"] not in (8, 32):
+        raise ValueError("state_bits must be 8 or 32, got %r" % (g["state_bits"],))
+      for p in g["params"]:
+        if id(p) in seen:
+          raise ValueError("a parameter appears more than once")
+        seen.add(id(p))
+    if not seen:
+      raise ValueError("AdamW got no parameters")
+    self._options()
+    self.max_grad_norm = max_grad_norm
+    self.seed = int(seed)
+    self._on_device = bool(capturable) or max_grad_norm is not None
+    self._buffers = None
+
+  def _options(self):
+    b1, b2 = self._uniform("betas")
+    eps = self._uniform("eps")
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+      raise ValueError("betas must be in [0, 1), got %r" % ((b1, b2),))
+    if not eps >= 0.0:
+      raise ValueError("eps must not be negative, got %r" % (eps,))
+    for g in self.param_groups:
+      if not torch.is_tensor(g["lr"]) and not g["lr"] >= 0.0:
+        raise ValueError("lr must not be negative, got %r" % (g["lr"],))
+      if not g["weight_decay"] >= 0.0:
+        raise ValueError("weight_decay must not be negative, got %r" % (g["weight_decay"],))
+    return b1, b2, eps
+
+  # ---- engine ---------------------------------------------------------------
+  covers = Adam.covers
+
+  def _attach(self, engine):
+    for key in ("lr", "weight_decay", "state_bits"):
+      self._uniform(key)
+    if self._buffers is not None:
+      raise RuntimeError("this AdamW has stepped parameters already: give OIVAE a new one")
+    super()._attach(engine)
+
+  def zero_grad(self, set_to_none=True):
+    """Drops the gradients (or, with set_to_none=False, zeroes them in place); nothing to do on an engine."""
+    if self._engine is not None:
+      return
+    for g in self.param_groups:
+      for p in g["params"]:
+        if set_to_none:
+          p.grad = None
+        elif p.grad is not None:
+          p.grad.detach_()
+          p.grad.zero_()
+
+  # ---- storage ---------------------------------------------------------------
+  def _setup(self):
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+      raise RuntimeError("AdamW allocates its moments at its first use: touch .buffers or take a step before capturing")
+    if self._engine is not None:
+      eng = self._engine
+      leaves, groups = [eng.flat_params[:eng.adam_numel]], [0]
+    else:
+      leaves = [p for g in self.param_groups for p in g["params"]]
+      groups = [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
+    device = _check_types(leaves, "parameters")
+    for p in leaves:
+      if not _dense(p):
+        raise ValueError("a parameter of strides %s and shape %s does not fill its memory" % (p.stride(), tuple(p.shape)))
+    self._leaves, self.device = leaves, device
+    self._lib = _lib.init_device(device.index)
+    index = np.arange(len(leaves))
+    self._kinds = []
+    buffers = {}
+    bits_of = np.array([self.param_groups[g]["state_bits"] for g in groups])
+    for bits in (32, 8):
+      # 16-bit parameters first: the master buffer need not reach further than they do
+      mine = sorted((int(i) for i in index[bits_of == bits]), key=lambda i: leaves[i].dtype == torch.float32)
+      if not mine:
+        continue
+      rec = np.zeros(len(mine), _TENSOR)
+      rec["n"] = [leaves[i].numel() for i in mine]
+      whole = (rec["n"] + _lib.ADAMW_BLOCK - 1) // _lib.ADAMW_BLOCK * _lib.ADAMW_BLOCK
+      rec["at"] = np.cumsum(whole) - whole
+      rec["p_type"] = [_TYPES[leaves[i].dtype] for i in mine]
+      rec["group"] = [groups[i] for i in mine]
+      rec["index"] = mine
+      total = int(whole.sum())
+      half = int(whole[rec["p_type"] != _lib.F32].sum())
+      held = {}
+      if bits == 32:
+        for name in ("exp_avg", "exp_avg_sq"):
+          held[name] = torch.zeros(total, dtype=torch.float32, device=device)
+      else:
+        for name, typ in (("exp_avg", torch.float8_e4m3fn), ("exp_avg_sq", torch.float8_e5m2)):
+          held[name] = torch.zeros(total, dtype=torch.uint8, device=device).view(typ)
+          held[name + "_scale"] = torch.zeros(total // _lib.ADAMW_BLOCK, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+      if half:
+        held["master"] = torch.zeros(half, dtype=torch.float32, device=device)
+      buffers[bits] = held
+      self._kinds.append((bits, mine, rec))
+    self._buffers = buffers
+    self._steps = np.zeros(len(leaves), np.int32)
+    self._steps_dev = torch.zeros(len(leaves), dtype=torch.int32, device=device) if self._on_device else None
+    self._clip = torch.zeros(4, dtype=torch.int32, device=device) if self._on_device else None
+    if self._on_device:
+      self._ws = torch.empty(self._lib.oivae_grad_norm_workspace_bytes(len(leaves)), dtype=torch.uint8, device=device)
+    self.sync_master()
+
+  @property
+  def buffers(self):
+    """The optimizer's state by number of bits: {32: {"exp_avg", "exp_avg_sq"[, "master"]}, 8: {"exp_avg", "exp_avg_scale",
+    "exp_avg_sq", "exp_avg_sq_scale"[, "master"]}}, flat tensors in which every parameter has a region of whole blocks of
+    128 elements (16-bit parameters first, else in the order given).  Allocated at first use."""
+    if self._buffers is None:
+      self._setup()
+    return self._buffers
+
+  def _views(self, name):
+    """(parameter, its part of the flat buffer `name`) of every parameter that has one, parameter by parameter."""
+    for bits, mine, rec in self._kinds:
+      flat = self._buffers[bits].get(name)
+      for i, r in zip(mine, rec):
+        if flat is not None and (name != "master" or r["p_type"] != _lib.F32):
+          yield self._leaves[i], flat[int(r["at"]):int(r["at"] + r["n"])]
+
+  @torch.no_grad()
+  def sync_master(self):
+    """Takes the master weights of 16-bit parameters from the parameters again."""
+    self.buffers
+    for p, flat in self._views("master"):
+      flat.as_strided(p.shape, p.stride()).copy_(p)
+
+  @property
+  def grad_norm(self):
+    """Norm of the last step's gradients (after grad_scale): a 0-dim tensor on the device.  Needs max_grad_norm."""
+    if self.max_grad_norm is None:
+      raise RuntimeError("AdamW computes the gradient norm where max_grad_norm is given")
+    self.buffers
+    return self._clip.view(torch.float32)[0]
+
+  @property
+  def skipped(self):
+    """Number of steps left out because their gradient norm was not finite: a 0-dim int32 tensor on the device."""
+    if not self._on_device:
+      raise RuntimeError("AdamW leaves steps out where max_grad_norm (or capturable) is given")
+    self.buffers
+    return self._clip[3]
+
+  def steps(self):
+    """Steps taken so far, parameter by parameter (a list; reads the device where the counts live there)."""
+    self.buffers
+    return (self._steps_dev if self._on_device else self._steps).tolist()
+
+  def set_steps(self, steps):
+    """Sets the step counts: one number for all parameters or one for each."""
+    self.buffers
+    counts = np.broadcast_to(np.asarray(steps, np.int32), self._steps.shape)
+    if (counts < 0).any():
+      raise ValueError("step counts must not be negative")
+    self._steps[:] = counts
+    if self._on_device:
+      self._steps_dev.copy_(torch.from_numpy(self._steps.copy()))
+
+  def state_dict(self):
+    """Everything a resumed run needs: counts, options and copies of `buffers`."""
+    return {"steps": self.steps(), "seed": self.seed,
+            "groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups],
+            "buffers": {bits: {k: t.clone() for k, t in held.items()} for bits, held in self.buffers.items()}}
+
+  @torch.no_grad()
+  def load_state_dict(self, state):
+    held = self.buffers
+    for what, mine, theirs in [("bits", held, state["buffers"])] + [("buffers", held[b], state["buffers"].get(b, {})) for b in held]:
+      if sorted(mine) != sorted(theirs):
+        raise ValueError("the state holds %s %s, this optimizer %s" % (what, sorted(theirs), sorted(mine)))
+    pairs = [(t, state["buffers"][b][k], k) for b in held for k, t in held[b].items()]
+    for t, src, k in pairs:
+      if src.shape != t.shape or src.dtype != t.dtype:
+        raise ValueError("%s is %s %s in the state, %s %s here" % (k, tuple(src.shape), src.dtype, tuple(t.shape), t.dtype))
+    if len(state["groups"]) != len(self.param_groups) or len(state["steps"]) != len(self._steps):
+      raise ValueError("the state was made for other parameter groups")
+    for t, src, _ in pairs:
+      t.view(torch.uint8).copy_(src.view(torch.uint8))
+    self.set_steps(state["steps"])
+    self.seed = state["seed"]
+    for g, src in zip(self.param_groups, state["groups"]):
+      g.update(src)
+
+  # ---- the step ---------------------------------------------------------------
+  def _gather(self):
+    """(index, gradient) of the tensors that take part, gradients in their parameter's order; pointers into the records."""
+    if self._engine is not None:
+      eng = self._engine
+      return self._leaves, [eng.flat_grads[:eng.adam_numel]]
+    leaves = self._leaves
+    grads = [p.grad for p in leaves]
+    for i, (p, g) in enumerate(zip(leaves, grads)):
+      if g is None:
+        continue
+      if g.layout != torch.strided:
+        raise ValueError("gradients must be dense tensors, got %s" % g.layout)
+      if g.dtype not in _TYPES or g.device != self.device or p.device != self.device:
+        raise ValueError("parameter and gradient must be float32, bfloat16 or float16 on %s, got %s on %s with %s on %s"
+                         % (self.device, p.dtype, p.device, g.dtype, g.device))
+      if g.shape != p.shape:
+        raise ValueError("a gradient of shape %s for a parameter of shape %s" % (tuple(g.shape), tuple(p.shape)))
+      if not (p.is_contiguous() and g.is_contiguous()):
+        if not _dense(p):
+          raise ValueError("a parameter of strides %s and shape %s does not fill its memory" % (p.stride(), tuple(p.shape)))
+        if g.stride() != p.stride():
+          grads[i] = torch.empty_like(p, dtype=g.dtype).copy_(g)   # in the parameter's order
+    return leaves, grads
+
+  @torch.no_grad()
+  def step(self, grad_scale=1.0):
+    """One step from the parameters' gradients, times grad_scale (1 / loss scale).  Parameters without a gradient stay as
+    they are and keep their count, as in torch.optim."""
+    b1, b2, eps = self._options()
+    if self._buffers is None:
+      self._setup()
+    L, dev = self._lib, self.device
+    with torch.cuda.device(dev):
+      if not self._on_device and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a captured step would repeat its step count at every replay: use AdamW(capturable=True)")
+      leaves, grads = self._gather()
+      take = np.array([g is not None for g in grads])
+      if not take.any():
+        return
+      groups = np.zeros(len(self.param_groups), _GROUP)
+      for q, g in zip(groups, self.param_groups):
+        if torch.is_tensor(g["lr"]):
+          if g["lr"].numel() != 1 or g["lr"].dtype != torch.float32 or g["lr"].device != dev:
+            raise ValueError("an lr tensor must be one float32 on %s" % dev)
+          q["lr_dev"] = g["lr"].data_ptr()
+        else:
+          q["lr"] = g["lr"]
+        q["weight_decay"] = g["weight_decay"]
+      stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+      todo = []
+      for bits, mine, rec in self._kinds:
+        for r, i in zip(rec, mine):
+          p, g = leaves[i], grads[i]
+          if g is None:
+            continue
+          if p.numel() != r["n"] or _TYPES.get(p.dtype) != r["p_type"]:
+            raise ValueError("a parameter changed its size or type since this optimizer's first step")
+          r["p"], r["g"], r["g_type"] = p.data_ptr(), g.data_ptr(), _TYPES[g.dtype]
+        keep = take[mine]
+        todo.append((bits, rec if keep.all() else rec[keep]))
+      clip = None
+      if self._on_device:
+        norm = np.zeros(int(take.sum()) if self.max_grad_norm is not None else 0, _GRAD)
+        which = np.concatenate([rec["index"] for _, rec in todo]).astype(np.int32)
+        if len(norm):
+          for src, dst in (("g", "g"), ("n", "n"), ("g_type", "type")):
+            norm[dst] = np.concatenate([rec[src] for _, rec in todo])
+        clip = self._clip.data_ptr()
+        _lib.check(L.oivae_grad_norm(norm.ctypes.data, len(norm), float(grad_scale), float(self.max_grad_norm or 0.0), clip,
+                                     self._steps_dev.data_ptr(), which.ctypes.data, len(which), self._ws.data_ptr(),
+                                     self._ws.numel(), stream), "oivae_grad_norm")
+      else:
+        self._steps[take] += 1
+      for bits, rec in todo:
+        if not len(rec):
+          continue
+        held = self._buffers[bits]
+        ptr = lambda k: held[k].data_ptr() if k in held else None
+        state = _lib.AdamwState(ptr("exp_avg"), ptr("exp_avg_sq"), ptr("exp_avg_scale"), ptr("exp_avg_sq_scale"), ptr("master"),
+                                self._steps_dev.data_ptr() if self._on_device else None)
+        rec["step"] = self._steps[rec["index"]]
+        args = (rec.ctypes.data, len(rec), groups.ctypes.data, len(groups), ctypes.byref(state), float(b1), float(b2), float(eps),
+                float(grad_scale))
+        if bits == 32:
+          _lib.check(L.oivae_adamw_f32(*args, clip, stream), "oivae_adamw_f32")
+        else:
+          _lib.check(L.oivae_adamw_f8(*args, self.seed, clip, stream), "oivae_adamw_f8")
