@@ -26,7 +26,7 @@ namespace oivae {
 //     accumulators stay in AGPRs through the builtin;
 //   * biases are folded into the accumulator's initial value (loaded from LDS),
 //     the tanh argument scale 2*log2(e) into a second copy of A;
-//   * all element-wise math is written on register pairs (v_pk_*_f32);
+//   * all element-wise math is written on register pairs;
 //   * column sums are accumulated as pairs and folded once at the end;
 //   * tile bookkeeping and the atomics' row bases are scalar (wave index through
 //     readfirstlane, 32-bit per-lane offsets).
@@ -44,9 +44,7 @@ __device__ __forceinline__ void mfv0(f32x16& acc, float a_, float b_) {
   asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 %0, %1, %2, 0" : "=&v"(acc) : "v"(a_), "v"(b_));
 }
 
-// AGPR form (weight-gradient accumulators, never touched by element-wise code).  Also inline asm: with no
-// MFMA visible to it, the compiler's gfx950 peephole that splits v_pk_*_f32 "in the shadow of an MFMA" into two
-// scalar VALU ops (right for bf16 MFMAs, wrong beside fp32 ones) leaves the packed element-wise math alone.
+// AGPR form (weight-gradient accumulators, never touched by element-wise code).  Also inline asm.
 __device__ __forceinline__ void mfa(f32x16& acc, float a_, float b_) {
   asm volatile("s_nop 1\n\tv_mfma_f32_32x32x2_f32 %0, %1, %2, %0" : "+a"(acc) : "v"(a_), "v"(b_));
 }
@@ -123,16 +121,9 @@ __device__ __forceinline__ void vphase2w(f32x16& acc0, f32x16& acc1, const float
 // never merged into ds_read2_b32, whose 8-bit offsets would cost one VALU add (8 matrix cycles) per merged pair.
 using ldsv_t = const volatile float __attribute__((address_space(3)))*;
 
-// Pins a value pair in a 64-bit register pair: the optimizer cannot scalarize arithmetic on it, so
-// the following vector ops select v_pk_*_f32 (one VALU slot for two floats).  Emits no instruction.
+// Pins a value pair in a 64-bit register pair (arithmetic on it stays two scalar instructions: the library is built
+// without the packed fp32 ones).  Emits no instruction.
 __device__ __forceinline__ f32x2 pin2(f32x2 v) { asm("" : "+v"(v)); return v; }
-// a - b on a register pair in ONE instruction (the compiler expands a v2f32 subtraction into two scalar ones)
-__device__ __forceinline__ f32x2 pk_sub(f32x2 a_, f32x2 b_) {
-  f32x2 r;
-  asm("v_pk_add_f32 %0, %1, %2 neg_lo:[0,1] neg_hi:[0,1]" : "=v"(r) : "v"(a_), "v"(b_));
-  return r;
-}
-
 __global__ __launch_bounds__(256) void dec_mfma64_v4(MfmaDecArgs a) {
   constexpr int K = 64, H = 64, M = 64, DG = 64;
   constexpr int LW = 65, LDB = 68;
@@ -293,7 +284,7 @@ __global__ __launch_bounds__(256) void dec_mfma64_v4(MfmaDecArgs a) {
         f32x2 mu = pin2(f32x2{gacc[t][4 * q + 2 * h2], gacc[t][4 * q + 2 * h2 + 1]});
         const f32x2 x = pin2(f32x2{xreg[t][q][2 * h2], xreg[t][q][2 * h2 + 1]});
         const f32x2 c = pin2(f32x2{c3[2 * h2], c3[2 * h2 + 1]});
-        mu = pin2(pk_sub(mu, x) * c);
+        mu = pin2((mu - x) * c);
         gacc[t][4 * q + 2 * h2] = mu[0]; gacc[t][4 * q + 2 * h2 + 1] = mu[1];
       }
       img_store(wrA, gacc[t], t, q);
