@@ -1,0 +1,140 @@
+// Reads lists of torch tensors into the records of the optimizer entry points (include/oivae_hip.h): addresses, sizes and
+// types of parameters and gradients.  In Python this costs about a microsecond a tensor and check, ten checks a tensor --
+// more than the kernels of a small model take; here a tensor costs about 20 ns.  Only the ordinary case is served: the
+// functions return the index of the first tensor that is anything else (another type, size, device or order than its
+// record says), and oi_vae_amd/optim.py then goes through the list itself, copies what can be copied and refuses the rest.
+#define PY_SSIZE_T_CLEAN
+#include <Python.h>
+
+#include <algorithm>
+#include <vector>
+
+#include <ATen/core/Tensor.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include "../../include/oivae_hip.h"
+
+namespace {
+
+int type_of(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return OIVAE_F32;
+    case at::kBFloat16: return OIVAE_BF16;
+    case at::kHalf: return OIVAE_F16;
+    default: return -1;
+  }
+}
+
+// one piece of device memory on `device`, its values as they stand
+bool plain(const at::Tensor& t, int device) {
+  return t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && !t.is_neg() && type_of(t) >= 0 &&
+         (t.is_contiguous() || t.is_non_overlapping_and_dense());
+}
+
+struct Buffer {
+  Py_buffer b;
+  bool held = false;
+  ~Buffer() { if (held) PyBuffer_Release(&b); }
+  bool take(PyObject* o, Py_ssize_t item, Py_ssize_t count) {
+    if (PyObject_GetBuffer(o, &b, PyBUF_WRITABLE | PyBUF_C_CONTIGUOUS) != 0) return false;
+    held = true;
+    if (b.len < item * count) {
+      PyErr_SetString(PyExc_ValueError, "fewer records than tensors");
+      return false;
+    }
+    return true;
+  }
+};
+
+// parameters(list, records of oivae_adamw_tensor_t, device, records of oivae_grad_t or None) -> (first unusual tensor or -1,
+// number without a gradient).  Fills p, g and g_type, g = 0 where a parameter has no gradient, and the gradients' records
+// (n = 0 there).  The records' n and p_type say what the parameters have to be.
+PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 4 || !PyList_Check(args[0])) {
+    PyErr_SetString(PyExc_TypeError, "parameters(list, records, device, gradient records)");
+    return nullptr;
+  }
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  Buffer buf, gbuf;
+  if (!buf.take(args[1], sizeof(oivae_adamw_tensor_t), n)) return nullptr;
+  const long device = PyLong_AsLong(args[2]);
+  if (device == -1 && PyErr_Occurred()) return nullptr;
+  if (args[3] != Py_None && !gbuf.take(args[3], sizeof(oivae_grad_t), n)) return nullptr;
+  oivae_adamw_tensor_t* r = static_cast<oivae_adamw_tensor_t*>(buf.b.buf);
+  oivae_grad_t* q = gbuf.held ? static_cast<oivae_grad_t*>(gbuf.b.buf) : nullptr;
+  long missing = 0;
+  Py_ssize_t unusual = -1;
+  try {
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* o = PyList_GET_ITEM(args[0], i);
+      unusual = i;
+      if (!THPVariable_Check(o)) break;
+      const at::Tensor& p = THPVariable_Unpack(o);
+      const at::Tensor& g = p.grad();
+      if (!g.defined()) {
+        r[i].g = nullptr;
+        if (q) q[i] = oivae_grad_t{nullptr, 0, OIVAE_F32, 0};
+        ++missing;
+        unusual = -1;
+        continue;
+      }
+      if (!plain(p, (int)device) || !plain(g, (int)device) || p.numel() != r[i].n || type_of(p) != r[i].p_type || !g.sizes().equals(p.sizes()))
+        break;
+      if (!(p.is_contiguous() && g.is_contiguous()) && !g.strides().equals(p.strides())) break;
+      r[i].p = p.data_ptr();
+      r[i].g = g.data_ptr();
+      r[i].g_type = type_of(g);
+      if (q) q[i] = oivae_grad_t{g.data_ptr(), g.numel(), type_of(g), 0};
+      unusual = -1;
+    }
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+  return Py_BuildValue("(nl)", unusual, missing);
+}
+
+// gradients(list, records of oivae_grad_t) -> (count, device) of the gradients that are there, or None when one is unusual,
+// appears twice or is on another device; (0, -1) without any.
+PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 2 || !PyList_Check(args[0])) {
+    PyErr_SetString(PyExc_TypeError, "gradients(list, records)");
+    return nullptr;
+  }
+  const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  Buffer buf;
+  if (!buf.take(args[1], sizeof(oivae_grad_t), n)) return nullptr;
+  oivae_grad_t* r = static_cast<oivae_grad_t*>(buf.b.buf);
+  long count = 0;
+  int device = -1;
+  try {
+    std::vector<void*> seen;
+    seen.reserve((size_t)n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      PyObject* o = PyList_GET_ITEM(args[0], i);
+      if (!THPVariable_Check(o)) Py_RETURN_NONE;
+      const at::Tensor& g = THPVariable_Unpack(o).grad();
+      if (!g.defined()) continue;
+      if (device < 0 && g.is_cuda()) device = (int)g.get_device();
+      if (!plain(g, device)) Py_RETURN_NONE;
+      r[count++] = oivae_grad_t{g.data_ptr(), g.numel(), type_of(g), 0};
+      if (g.numel() > 0) seen.push_back(g.data_ptr());
+    }
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+  return Py_BuildValue("(li)", count, device);
+}
+
+PyMethodDef methods[] = {
+    {"parameters", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(parameters)), METH_FASTCALL, nullptr},
+    {"gradients", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gradients)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_lists", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__tensor_lists(void) { return PyModule_Create(&module); }

@@ -110,8 +110,8 @@ _GROUP = np.dtype([("lr", "f4"), ("weight_decay", "f4"), ("lr_dev", "u8")])     
 
 
 def _dense(t):
-  """Whether t's elements fill one piece of memory, in any order of its dimensions."""
-  if t.layout != torch.strided:
+  """Whether t's elements fill one piece of memory as they stand, in any order of its dimensions."""
+  if t.layout != torch.strided or t.is_neg():
     return False
   expect = 1
   for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
@@ -136,39 +136,66 @@ def _check_types(tensors, what):
   return device
 
 
+def _lists():
+  """The native reader of tensor lists (csrc/tensor_lists.cpp)."""
+  global _lists_module
+  if _lists_module is None:
+    try:
+      from . import _tensor_lists
+    except ImportError as e:
+      raise _lib.OivaeError("oi_vae_amd/_tensor_lists.so is not built (%s): run `make -C oi_vae_amd/csrc`" % e)
+    _lists_module = _tensor_lists
+  return _lists_module
+
+
+_lists_module = None
+
+
 def _grads_of(parameters):
+  """(records, device index, gradients, their dense copies where they are not one piece of memory) of the gradients that
+  are there; None without any."""
   ps = [parameters] if torch.is_tensor(parameters) else list(parameters)
+  rec = np.zeros(len(ps), _GRAD)
+  got = _lists().gradients(ps, rec)
+  if got is not None:
+    count, device = got
+    return (rec[:count], device, (), ()) if count else None
   grads = [p.grad for p in ps if p.grad is not None]
   device = _check_types(grads, "gradients")
   if len({g.data_ptr() for g in grads if g.numel()}) != sum(1 for g in grads if g.numel()):
     raise ValueError("the same gradient appears more than once")
-  return grads, device
-
-
-def _norm_of(grads, device, max_norm):
-  L = _lib.init_device(device.index)
+  with torch.no_grad():
+    packed = [g if _dense(g) else torch.empty(g.shape, dtype=g.dtype, device=device).copy_(g) for g in grads]
   rec = np.zeros(len(grads), _GRAD)
-  rec["g"] = [g.data_ptr() for g in grads]
-  rec["n"] = [g.numel() for g in grads]
-  rec["type"] = [_TYPES[g.dtype] for g in grads]
-  clip = torch.zeros(4, dtype=torch.float32, device=device)
-  nbytes = L.oivae_grad_norm_workspace_bytes(len(grads))
-  ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-  stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-  _lib.check(L.oivae_grad_norm(rec.ctypes.data, len(grads), 1.0, max_norm, clip.data_ptr(), None, None, 0, ws.data_ptr(), nbytes,
-                               stream), "oivae_grad_norm")
-  return L, rec, clip, stream
+  rec["g"] = [g.data_ptr() for g in packed]
+  rec["n"] = [g.numel() for g in packed]
+  rec["type"] = [_TYPES[g.dtype] for g in packed]
+  return rec, device.index, grads, packed
+
+
+def _norm_of(rec, device, max_norm, scale):
+  L = _lib.init_device(device)
+  nbytes = L.oivae_grad_norm_workspace_bytes(len(rec))
+  # verdict (16 bytes, written whole) and workspace of this call alone: calls on other streams and in captured graphs have
+  # their own
+  ws = torch.empty(nbytes // 4 + 4, dtype=torch.float32, device=torch.device("cuda", device))
+  clip, address = ws.data_ptr(), rec.ctypes.data
+  stream = torch.cuda.current_stream(device).cuda_stream
+  _lib.check(L.oivae_grad_norm(address, len(rec), 1.0, max_norm, clip, None, None, 0, clip + 16, nbytes, stream), "oivae_grad_norm")
+  if scale:
+    _lib.check(L.oivae_grad_clip(address, len(rec), clip, stream), "oivae_grad_clip")
+  return ws[0]
 
 
 def grad_norm(parameters):
   """2-norm of the gradients of `parameters` (a tensor or an iterable of tensors; those without a gradient are left out)
   taken as one vector: a 0-dim float32 tensor on their device, with no synchronisation.  Squares and sums are formed in
   fp64, in an order that depends on the sizes alone."""
-  grads, device = _grads_of(parameters)
-  if not grads:
+  got = _grads_of(parameters)
+  if got is None:
     return torch.zeros(())
-  with torch.cuda.device(device):
-    return _norm_of([g if _dense(g) else g.contiguous() for g in grads], device, 0.0)[2][0]
+  with torch.cuda.device(got[1]):
+    return _norm_of(got[0], got[1], 0.0, False)
 
 
 def clip_grad_norm_(parameters, max_norm):
@@ -177,17 +204,17 @@ def clip_grad_norm_(parameters, max_norm):
   max_norm = float(max_norm)
   if not max_norm > 0:
     raise ValueError("max_norm must be positive, got %r" % max_norm)
-  grads, device = _grads_of(parameters)
-  if not grads:
+  got = _grads_of(parameters)
+  if got is None:
     return torch.zeros(())
+  rec, device, grads, packed = got
   with torch.cuda.device(device):
-    packed = [g if _dense(g) else g.contiguous() for g in grads]
-    L, rec, clip, stream = _norm_of(packed, device, max_norm)
-    _lib.check(L.oivae_grad_clip(rec.ctypes.data, len(packed), clip.data_ptr(), stream), "oivae_grad_clip")
-    for g, c in zip(grads, packed):
-      if c is not g:
-        g.copy_(c)
-    return clip[0]
+    norm = _norm_of(rec, device, max_norm, True)
+    with torch.no_grad():
+      for g, c in zip(grads, packed):
+        if c is not g:
+          g.copy_(c)
+  return norm
 
 
 class AdamW(_EngineOptimizer):
@@ -283,42 +310,26 @@ class AdamW(_EngineOptimizer):
         raise ValueError("a parameter of strides %s and shape %s does not fill its memory" % (p.stride(), tuple(p.shape)))
     self._leaves, self.device = leaves, device
     self._lib = _lib.init_device(device.index)
-    index = np.arange(len(leaves))
     self._kinds = []
-    buffers = {}
-    bits_of = np.array([self.param_groups[g]["state_bits"] for g in groups])
+    self._steps_dev = torch.zeros(len(leaves), dtype=torch.int32, device=device) if self._on_device else None
+    bits_of = [self.param_groups[g]["state_bits"] for g in groups]
     for bits in (32, 8):
       # 16-bit parameters first: the master buffer need not reach further than they do
-      mine = sorted((int(i) for i in index[bits_of == bits]), key=lambda i: leaves[i].dtype == torch.float32)
-      if not mine:
-        continue
-      rec = np.zeros(len(mine), _TENSOR)
-      rec["n"] = [leaves[i].numel() for i in mine]
-      whole = (rec["n"] + _lib.ADAMW_BLOCK - 1) // _lib.ADAMW_BLOCK * _lib.ADAMW_BLOCK
-      rec["at"] = np.cumsum(whole) - whole
-      rec["p_type"] = [_TYPES[leaves[i].dtype] for i in mine]
-      rec["group"] = [groups[i] for i in mine]
-      rec["index"] = mine
-      total = int(whole.sum())
-      half = int(whole[rec["p_type"] != _lib.F32].sum())
-      held = {}
-      if bits == 32:
-        for name in ("exp_avg", "exp_avg_sq"):
-          held[name] = torch.zeros(total, dtype=torch.float32, device=device)
-      else:
-        for name, typ in (("exp_avg", torch.float8_e4m3fn), ("exp_avg_sq", torch.float8_e5m2)):
-          held[name] = torch.zeros(total, dtype=torch.uint8, device=device).view(typ)
-          held[name + "_scale"] = torch.zeros(total // _lib.ADAMW_BLOCK, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
-      if half:
-        held["master"] = torch.zeros(half, dtype=torch.float32, device=device)
-      buffers[bits] = held
-      self._kinds.append((bits, mine, rec))
-    self._buffers = buffers
-    self._steps = np.zeros(len(leaves), np.int32)
-    self._steps_dev = torch.zeros(len(leaves), dtype=torch.int32, device=device) if self._on_device else None
+      mine = sorted((i for i in range(len(leaves)) if bits_of[i] == bits), key=lambda i: leaves[i].dtype == torch.float32)
+      if mine:
+        self._kinds.append(_Kind(self, bits, mine, groups))
+    buffers = {k.bits: k.held for k in self._kinds}
     self._clip = torch.zeros(4, dtype=torch.int32, device=device) if self._on_device else None
     if self._on_device:
       self._ws = torch.empty(self._lib.oivae_grad_norm_workspace_bytes(len(leaves)), dtype=torch.uint8, device=device)
+      # gradients' records and step counters of all kinds, one behind the other
+      self._norm_rec = np.zeros(len(leaves), _GRAD)
+      self._which = np.concatenate([k.rec["index"] for k in self._kinds]).astype(np.int32)
+      at = 0
+      for k in self._kinds:
+        k.grads = self._norm_rec[at:at + len(k.mine)]
+        at += len(k.mine)
+    self._buffers = buffers
     self.sync_master()
 
   @property
@@ -332,9 +343,9 @@ class AdamW(_EngineOptimizer):
 
   def _views(self, name):
     """(parameter, its part of the flat buffer `name`) of every parameter that has one, parameter by parameter."""
-    for bits, mine, rec in self._kinds:
-      flat = self._buffers[bits].get(name)
-      for i, r in zip(mine, rec):
+    for k in self._kinds:
+      flat = k.held.get(name)
+      for i, r in zip(k.mine, k.rec):
         if flat is not None and (name != "master" or r["p_type"] != _lib.F32):
           yield self._leaves[i], flat[int(r["at"]):int(r["at"] + r["n"])]
 
@@ -364,17 +375,23 @@ class AdamW(_EngineOptimizer):
   def steps(self):
     """Steps taken so far, parameter by parameter (a list; reads the device where the counts live there)."""
     self.buffers
-    return (self._steps_dev if self._on_device else self._steps).tolist()
+    if self._on_device:
+      return self._steps_dev.tolist()
+    counts = np.zeros(len(self._leaves), np.int32)
+    for k in self._kinds:
+      counts[k.mine] = k.rec["step"]
+    return counts.tolist()
 
   def set_steps(self, steps):
     """Sets the step counts: one number for all parameters or one for each."""
     self.buffers
-    counts = np.broadcast_to(np.asarray(steps, np.int32), self._steps.shape)
+    counts = np.broadcast_to(np.asarray(steps, np.int32), (len(self._leaves),))
     if (counts < 0).any():
       raise ValueError("step counts must not be negative")
-    self._steps[:] = counts
+    for k in self._kinds:
+      k.rec["step"] = counts[k.mine]
     if self._on_device:
-      self._steps_dev.copy_(torch.from_numpy(self._steps.copy()))
+      self._steps_dev.copy_(torch.from_numpy(counts.copy()))
 
   def state_dict(self):
     """Everything a resumed run needs: counts, options and copies of `buffers`."""
@@ -392,7 +409,7 @@ class AdamW(_EngineOptimizer):
     for t, src, k in pairs:
       if src.shape != t.shape or src.dtype != t.dtype:
         raise ValueError("%s is %s %s in the state, %s %s here" % (k, tuple(src.shape), src.dtype, tuple(t.shape), t.dtype))
-    if len(state["groups"]) != len(self.param_groups) or len(state["steps"]) != len(self._steps):
+    if len(state["groups"]) != len(self.param_groups) or len(state["steps"]) != len(self._leaves):
       raise ValueError("the state was made for other parameter groups")
     for t, src, _ in pairs:
       t.view(torch.uint8).copy_(src.view(torch.uint8))
@@ -402,90 +419,133 @@ class AdamW(_EngineOptimizer):
       g.update(src)
 
   # ---- the step ---------------------------------------------------------------
-  def _gather(self):
-    """(index, gradient) of the tensors that take part, gradients in their parameter's order; pointers into the records."""
-    if self._engine is not None:
-      eng = self._engine
-      return self._leaves, [eng.flat_grads[:eng.adam_numel]]
-    leaves = self._leaves
-    grads = [p.grad for p in leaves]
-    for i, (p, g) in enumerate(zip(leaves, grads)):
+  def _read(self, kind, copies):
+    """Addresses of a kind's parameters and gradients into its records, the way round (csrc/tensor_lists.cpp takes lists
+    that are all as their records say): copies gradients into their parameter's order, says what cannot be stepped.
+    Returns the number without a gradient; the copies, which have to live until the step is queued, go into `copies`."""
+    missing = 0
+    for j, i in enumerate(kind.mine):
+      p, r = self._leaves[i], kind.rec[j]
+      g = p.grad
       if g is None:
+        r["g"], missing = 0, missing + 1
+        if kind.grads is not None:
+          kind.grads[j] = (0, 0, 0, 0)
         continue
       if g.layout != torch.strided:
         raise ValueError("gradients must be dense tensors, got %s" % g.layout)
       if g.dtype not in _TYPES or g.device != self.device or p.device != self.device:
         raise ValueError("parameter and gradient must be float32, bfloat16 or float16 on %s, got %s on %s with %s on %s"
                          % (self.device, p.dtype, p.device, g.dtype, g.device))
+      if p.numel() != r["n"] or _TYPES.get(p.dtype) != r["p_type"]:
+        raise ValueError("a parameter changed its size or type since this optimizer's first step")
       if g.shape != p.shape:
         raise ValueError("a gradient of shape %s for a parameter of shape %s" % (tuple(g.shape), tuple(p.shape)))
-      if not (p.is_contiguous() and g.is_contiguous()):
-        if not _dense(p):
-          raise ValueError("a parameter of strides %s and shape %s does not fill its memory" % (p.stride(), tuple(p.shape)))
-        if g.stride() != p.stride():
-          grads[i] = torch.empty_like(p, dtype=g.dtype).copy_(g)   # in the parameter's order
-    return leaves, grads
+      if not _dense(p):
+        raise ValueError("a parameter of strides %s and shape %s does not fill its memory" % (p.stride(), tuple(p.shape)))
+      if g.is_neg() or (g.stride() != p.stride() and not (p.is_contiguous() and g.is_contiguous())):
+        g = torch.empty_like(p, dtype=g.dtype).copy_(g)
+        copies.append(g)
+      r["p"], r["g"], r["g_type"] = p.data_ptr(), g.data_ptr(), _TYPES[g.dtype]
+      if kind.grads is not None:
+        kind.grads[j] = (g.data_ptr(), g.numel(), _TYPES[g.dtype], 0)
+    return missing
 
   @torch.no_grad()
   def step(self, grad_scale=1.0):
     """One step from the parameters' gradients, times grad_scale (1 / loss scale).  Parameters without a gradient stay as
     they are and keep their count, as in torch.optim."""
-    b1, b2, eps = self._options()
     if self._buffers is None:
       self._setup()
-    L, dev = self._lib, self.device
-    with torch.cuda.device(dev):
-      if not self._on_device and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("a captured step would repeat its step count at every replay: use AdamW(capturable=True)")
-      leaves, grads = self._gather()
-      take = np.array([g is not None for g in grads])
-      if not take.any():
-        return
-      groups = np.zeros(len(self.param_groups), _GROUP)
-      for q, g in zip(groups, self.param_groups):
-        if torch.is_tensor(g["lr"]):
-          if g["lr"].numel() != 1 or g["lr"].dtype != torch.float32 or g["lr"].device != dev:
-            raise ValueError("an lr tensor must be one float32 on %s" % dev)
-          q["lr_dev"] = g["lr"].data_ptr()
-        else:
-          q["lr"] = g["lr"]
-        q["weight_decay"] = g["weight_decay"]
-      stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-      todo = []
-      for bits, mine, rec in self._kinds:
-        for r, i in zip(rec, mine):
-          p, g = leaves[i], grads[i]
-          if g is None:
-            continue
-          if p.numel() != r["n"] or _TYPES.get(p.dtype) != r["p_type"]:
-            raise ValueError("a parameter changed its size or type since this optimizer's first step")
-          r["p"], r["g"], r["g_type"] = p.data_ptr(), g.data_ptr(), _TYPES[g.dtype]
-        keep = take[mine]
-        todo.append((bits, rec if keep.all() else rec[keep]))
-      clip = None
-      if self._on_device:
-        norm = np.zeros(int(take.sum()) if self.max_grad_norm is not None else 0, _GRAD)
-        which = np.concatenate([rec["index"] for _, rec in todo]).astype(np.int32)
-        if len(norm):
-          for src, dst in (("g", "g"), ("n", "n"), ("g_type", "type")):
-            norm[dst] = np.concatenate([rec[src] for _, rec in todo])
-        clip = self._clip.data_ptr()
-        _lib.check(L.oivae_grad_norm(norm.ctypes.data, len(norm), float(grad_scale), float(self.max_grad_norm or 0.0), clip,
-                                     self._steps_dev.data_ptr(), which.ctypes.data, len(which), self._ws.data_ptr(),
-                                     self._ws.numel(), stream), "oivae_grad_norm")
+    if torch.cuda.current_device() == self.device.index:
+      self._step(float(grad_scale))
+    else:
+      with torch.cuda.device(self.device):
+        self._step(float(grad_scale))
+
+  def _step(self, grad_scale):
+    (b1, b2), eps = self._uniform("betas"), self._uniform("eps")
+    L, index = self._lib, self.device.index
+    if not self._on_device and torch.cuda.is_current_stream_capturing():
+      raise RuntimeError("a captured step would repeat its step count at every replay: use AdamW(capturable=True)")
+    groups = np.array([self._group_options(g) for g in self.param_groups], _GROUP)
+    todo, partial, copies = [], False, []
+    for k in self._kinds:
+      if self._engine is not None:
+        k.rec["p"], k.rec["g"] = self._leaves[0].data_ptr(), self._engine.flat_grads.data_ptr()
+        if k.grads is not None:
+          k.grads[0] = (k.rec["g"][0], k.rec["n"][0], _lib.F32, 0)
+        missing = 0
       else:
-        self._steps[take] += 1
-      for bits, rec in todo:
-        if not len(rec):
-          continue
-        held = self._buffers[bits]
-        ptr = lambda k: held[k].data_ptr() if k in held else None
-        state = _lib.AdamwState(ptr("exp_avg"), ptr("exp_avg_sq"), ptr("exp_avg_scale"), ptr("exp_avg_sq_scale"), ptr("master"),
-                                self._steps_dev.data_ptr() if self._on_device else None)
-        rec["step"] = self._steps[rec["index"]]
-        args = (rec.ctypes.data, len(rec), groups.ctypes.data, len(groups), ctypes.byref(state), float(b1), float(b2), float(eps),
-                float(grad_scale))
-        if bits == 32:
-          _lib.check(L.oivae_adamw_f32(*args, clip, stream), "oivae_adamw_f32")
+        unusual, missing = _lists().parameters(k.leaves, k.rec, index, k.grads)
+        if unusual >= 0:
+          missing = self._read(k, copies)
+      rec = k.rec
+      if missing:
+        partial, rec = True, rec[rec["g"] != 0]
+      todo.append((k, rec))
+    if partial and not any(len(rec) for _, rec in todo):
+      return
+    stream = torch.cuda.current_stream(index).cuda_stream
+    clip = None
+    if self._on_device:
+      which = self._which
+      if partial:
+        which = np.concatenate([rec["index"] for _, rec in todo])
+      clip = self._clip.data_ptr()
+      norm = self.max_grad_norm
+      _lib.check(L.oivae_grad_norm(self._norm_rec.ctypes.data, 0 if norm is None else len(self._norm_rec), grad_scale,
+                                   0.0 if norm is None else float(norm), clip, self._steps_dev.data_ptr(), which.ctypes.data,
+                                   len(which), self._ws.data_ptr(), self._ws.numel(), stream), "oivae_grad_norm")
+    for k, rec in todo:
+      if not len(rec):
+        continue
+      if not self._on_device:
+        if rec is k.rec:
+          rec["step"] += 1
         else:
-          _lib.check(L.oivae_adamw_f8(*args, self.seed, clip, stream), "oivae_adamw_f8")
+          k.rec["step"][k.rec["g"] != 0] += 1
+          rec["step"] += 1
+      args = (rec.ctypes.data, len(rec), groups.ctypes.data, len(groups), k.state_ref, b1, b2, eps, grad_scale)
+      if k.bits == 32:
+        _lib.check(L.oivae_adamw_f32(*args, clip, stream), "oivae_adamw_f32")
+      else:
+        _lib.check(L.oivae_adamw_f8(*args, self.seed, clip, stream), "oivae_adamw_f8")
+
+  def _group_options(self, g):
+    lr = g["lr"]
+    if not torch.is_tensor(lr):
+      return lr, g["weight_decay"], 0
+    if lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != self.device:
+      raise ValueError("an lr tensor must be one float32 on %s" % self.device)
+    return 0.0, g["weight_decay"], lr.data_ptr()
+
+
+class _Kind(object):
+  """The parameters of one AdamW whose moments have one number of bits: their records and flat buffers."""
+
+  def __init__(self, opt, bits, mine, groups):
+    leaves, device = opt._leaves, opt.device
+    self.bits, self.mine, self.leaves, self.grads = bits, mine, [leaves[i] for i in mine], None
+    self.rec = rec = np.zeros(len(mine), _TENSOR)
+    rec["n"] = [p.numel() for p in self.leaves]
+    whole = (rec["n"] + _lib.ADAMW_BLOCK - 1) // _lib.ADAMW_BLOCK * _lib.ADAMW_BLOCK
+    rec["at"] = np.cumsum(whole) - whole
+    rec["p_type"] = [_TYPES[p.dtype] for p in self.leaves]
+    rec["group"] = [groups[i] for i in mine]
+    rec["index"] = mine
+    total, half = max(int(whole.sum()), _lib.ADAMW_BLOCK), int(whole[rec["p_type"] != _lib.F32].sum())
+    self.held = held = {}
+    if bits == 32:
+      for name in ("exp_avg", "exp_avg_sq"):
+        held[name] = torch.zeros(total, dtype=torch.float32, device=device)
+    else:
+      for name, typ in (("exp_avg", torch.float8_e4m3fn), ("exp_avg_sq", torch.float8_e5m2)):
+        held[name] = torch.zeros(total, dtype=torch.uint8, device=device).view(typ)
+        held[name + "_scale"] = torch.zeros(total // _lib.ADAMW_BLOCK, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+    if half:
+      held["master"] = torch.zeros(half, dtype=torch.float32, device=device)
+    ptr = lambda k: held[k].data_ptr() if k in held and held[k].numel() else None
+    self.state = _lib.AdamwState(ptr("exp_avg"), ptr("exp_avg_sq"), ptr("exp_avg_scale"), ptr("exp_avg_sq_scale"), ptr("master"),
+                                 opt._steps_dev.data_ptr() if opt._on_device else None)
+    self.state_ref = ctypes.byref(self.state)

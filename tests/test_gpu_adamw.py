@@ -38,7 +38,8 @@ def _opt(groups, t, seed=0, **kw):
   opt = optim.AdamW(groups, betas=(B1, B2), eps=EPS, **kw)
   rng = np.random.default_rng(seed)
   opt.buffers
-  for bits, mine, rec in opt._kinds:
+  for k in opt._kinds:
+    bits, mine, rec = k.bits, k.mine, k.rec
     held = opt.buffers[bits]
     for r in rec:
       a, n = int(r["at"]), int(r["n"])
@@ -63,7 +64,8 @@ def _state(opt):
   """Per parameter: (w, m, v) as float64 arrays in the flat order, and the codes and scale bytes of 8-bit moments."""
   out = {}
   opt.buffers
-  for bits, mine, rec in opt._kinds:
+  for k in opt._kinds:
+    bits, mine, rec = k.bits, k.mine, k.rec
     held = opt.buffers[bits]
     for i, r in zip(mine, rec):
       a, n = int(r["at"]), int(r["n"])
