@@ -276,16 +276,26 @@ typedef struct {
   void* g;          /* device */
   int64_t n;
   int32_t type;     /* OIVAE_F32 | OIVAE_BF16 | OIVAE_F16 */
-  int32_t pad;
+  int32_t index;    /* of its step counter; -1: none */
 } oivae_grad_t;
 
-/* Verdict of oivae_grad_norm, on the device; zero it once before its first use. */
+/* Verdict of oivae_grad_norm, on the device; zero it once before its first use.  Calls that share one follow each other on
+ * one stream. */
 typedef struct {
   float norm, coef;
   int32_t skip;      /* 1: the norm is not finite (or a decoder launch behind the gradients failed): oivae_adamw_* leave
                         everything untouched */
   int32_t skipped;   /* steps left out so far (counted where step counters are given) */
+  uint32_t ticket;   /* the library's */
+  int32_t pad[3];
 } oivae_clip_t;
+
+/* A step counter on the device, with the bias corrections of that step; zero it once. */
+typedef struct {
+  int32_t t;                      /* steps taken, the current one included */
+  float inv_bc1, inv_bc2_sqrt;    /* 1 / (1 - b1^t), 1 / sqrt(1 - b2^t) */
+  int32_t pad;
+} oivae_step_t;
 
 typedef struct {
   void* p;           /* parameter (device) */
@@ -314,19 +324,20 @@ typedef struct {
   uint8_t* m_scale;
   uint8_t* v_scale;
   float* master;         /* fp32 weights of the 16-bit parameters; may be NULL when there are none */
-  const int32_t* steps;  /* step counters by tensor index, as oivae_grad_norm left them; NULL: the tensors' own `step` */
+  const oivae_step_t* steps;  /* step counters by tensor index, as oivae_grad_norm left them; NULL: the tensors' own `step` */
 } oivae_adamw_state_t;
 
-/* Norm, coefficient and verdict into `clip`; then, unless the step is to be left out, steps[which[i]] += 1 for the
- * n_which counters named (host array; steps may be NULL with n_which = 0).  count = 0 gives norm 0.
+/* Norm (with_norm = 0: not computed, zero), coefficient and verdict into `clip`; then, where `steps` is given and the step is
+ * not to be left out, the counters of the tensors advance (distinct indices), with the corrections for beta1 and beta2.
  * workspace: oivae_grad_norm_workspace_bytes(count) bytes on the device, 8-byte aligned. */
 int64_t oivae_grad_norm_workspace_bytes(int32_t count);
-int oivae_grad_norm(const oivae_grad_t* grads, int32_t count, float grad_scale, float max_norm, oivae_clip_t* clip,
-                    int32_t* steps, const int32_t* which, int32_t n_which, void* workspace, int64_t workspace_bytes,
-                    void* stream);
+int oivae_grad_norm(const oivae_grad_t* grads, int32_t count, int32_t with_norm, float grad_scale, float max_norm,
+                    oivae_clip_t* clip, oivae_step_t* steps, double beta1, double beta2, void* workspace,
+                    int64_t workspace_bytes, void* stream);
 
-/* g *= clip->coef in place (nothing is touched when it is 1). */
-int oivae_grad_clip(const oivae_grad_t* grads, int32_t count, const oivae_clip_t* clip, void* stream);
+/* Norm into *norm (device), then g *= coef in place (max_norm <= 0, or a coefficient of 1: nothing is touched). */
+int oivae_clip_grad_norm(const oivae_grad_t* grads, int32_t count, float max_norm, float* norm, void* workspace,
+                         int64_t workspace_bytes, void* stream);
 
 /* One AdamW step of `count` tensors; `clip` (may be NULL) from oivae_grad_norm on the same stream. */
 int oivae_adamw_f32(const oivae_adamw_tensor_t* tensors, int32_t count, const oivae_adamw_group_t* groups, int32_t n_groups,

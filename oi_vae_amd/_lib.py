@@ -25,7 +25,7 @@ SYMBOLS = [
   "oivae_adam_f32", "oivae_encoder_bwd_noalloc_f32", "oivae_dz_layout", "oivae_reload_test_hooks",
   "oivae_check_errors", "oivae_small_step_applies", "oivae_small_step_f32",
   "oivae_gamma_workspace_bytes", "oivae_gamma_logprob_f32",
-  "oivae_grad_norm_workspace_bytes", "oivae_grad_norm", "oivae_grad_clip", "oivae_adamw_f32", "oivae_adamw_f8",
+  "oivae_grad_norm_workspace_bytes", "oivae_grad_norm", "oivae_clip_grad_norm", "oivae_adamw_f32", "oivae_adamw_f8",
 ]
 
 F32, BF16, F16 = 0, 1, 2     # element types of the optimizer operators over lists of tensors
@@ -105,13 +105,13 @@ def bind(path):
   L.oivae_gamma_logprob_f32.restype = ctypes.c_int
   L.oivae_grad_norm_workspace_bytes.argtypes = [c_i32]
   L.oivae_grad_norm_workspace_bytes.restype = c_i64
-  L.oivae_grad_norm.argtypes = [c_vp, c_i32, c_f, c_f, c_vp, c_vp, c_vp, c_i32, c_vp, c_i64, c_vp]
-  L.oivae_grad_clip.argtypes = [c_vp, c_i32, c_vp, c_vp]
+  L.oivae_grad_norm.argtypes = [c_vp, c_i32, c_i32, c_f, c_f, c_vp, c_vp, ctypes.c_double, ctypes.c_double, c_vp, c_i64, c_vp]
+  L.oivae_clip_grad_norm.argtypes = [c_vp, c_i32, c_f, c_vp, c_vp, c_i64, c_vp]
   L.oivae_adamw_f32.argtypes = [c_vp, c_i32, c_vp, c_i32, ctypes.POINTER(AdamwState), ctypes.c_double, ctypes.c_double,
                                 ctypes.c_double, c_f, c_vp, c_vp]
   L.oivae_adamw_f8.argtypes = [c_vp, c_i32, c_vp, c_i32, ctypes.POINTER(AdamwState), ctypes.c_double, ctypes.c_double,
                                ctypes.c_double, c_f, ctypes.c_uint32, c_vp, c_vp]
-  for name in ("oivae_grad_norm", "oivae_grad_clip", "oivae_adamw_f32", "oivae_adamw_f8"):
+  for name in ("oivae_grad_norm", "oivae_clip_grad_norm", "oivae_adamw_f32", "oivae_adamw_f8"):
     getattr(L, name).restype = ctypes.c_int
   L.oivae_reload_test_hooks.argtypes = []
   L.oivae_reload_test_hooks.restype = None

@@ -13,20 +13,22 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace oivae {
 
 constexpr int kThreads = 256;
 constexpr int kMomentBlock = OIVAE_ADAMW_BLOCK;   // a tensor's moments occupy whole blocks of 128 elements
 constexpr int kSlots = 76;        // tensors of one AdamW launch: the argument struct stays below 4 KiB
-constexpr int kGroups = 8;        // (lr, decay) pairs of one launch
+constexpr int kOptions = 8;       // sets of (lr, decay, step) in one launch
+constexpr int kChunk = 1024;      // elements of an AdamW workgroup: one vector of four a thread
 constexpr int kGradSlots = 160;   // tensors of one norm / scaling launch
-constexpr int kNormBlocks = 1024; // cap on the blocks of one norm launch (= its partial sums)
-constexpr int kAdvance = 896;     // step counters advanced by one launch
+constexpr int kNormBlocks = 2048; // cap on the blocks of one norm launch (= its partial sums)
+constexpr int kFewBlocks = 256;   // up to so many, the norm is concluded without a launch of its own
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));        // parameters and gradients may start anywhere
 typedef uint16_t h4u __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef float f2v __attribute__((vector_size(8)));
 
 // ---- types of gradients and parameters ---------------------------------------------------------------------------------
@@ -100,19 +102,44 @@ __device__ __forceinline__ void store4(void* p, int type, int64_t i, int64_t n, 
   }
 }
 
+// weights and moments: read once and written once a step, past the caches that the gradients -- just written by the backward
+// pass -- may still be in
+__device__ __forceinline__ f4 stream4(const float* p, int64_t i, int64_t n) {
+  if (i + 4 <= n) return __builtin_nontemporal_load(reinterpret_cast<const f4u*>(p + i));
+  return load4(p, OIVAE_F32, i, n);
+}
+
+__device__ __forceinline__ void stream4(float* p, int64_t i, int64_t n, f4 x) {
+  if (i + 4 <= n) __builtin_nontemporal_store((f4u)x, reinterpret_cast<f4u*>(p + i));
+  else store4(p, OIVAE_F32, i, n, x);
+}
+
+__device__ __forceinline__ void stream4_half(void* p, int type, int64_t i, int64_t n, f4 x) {
+  if (i + 4 > n) {
+    store4(p, type, i, n, x);
+    return;
+  }
+  h4u h;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = float_to_half(x[j], type);
+  __builtin_nontemporal_store(h, reinterpret_cast<h4u*>(static_cast<uint16_t*>(p) + i));
+}
+
 // ---- gradient norm -----------------------------------------------------------------------------------------------------
 struct GradSlot {
   void* g;
   int64_t n;
   uint32_t first;   // its first chunk in the launch
-  int32_t type;
+  uint32_t info;    // type | (index of its step counter + 1) << 2
 };
 struct GradLaunch {
   GradSlot s[kGradSlots];
   int32_t count;
   uint32_t chunks;
 };
-constexpr int kGradChunk = 4096;   // elements
+
+// elements of one chunk: 256 threads x four vectors of 16 bytes
+__host__ __device__ inline int grad_chunk(int type) { return type == OIVAE_F32 ? 4096 : 8192; }
 
 // the last slot whose first chunk is not behind `chunk`
 template <class Launch>
@@ -125,10 +152,12 @@ __device__ __forceinline__ int find_slot(const Launch& a, uint32_t chunk) {
   return lo;
 }
 
+// the same sum in every thread, in an order of its own: within waves, then over waves
 __device__ __forceinline__ double block_sum(double x) {
   __shared__ double part[kThreads / 64];
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  __syncthreads();
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
   __syncthreads();
   double s = 0.0;
@@ -137,71 +166,187 @@ __device__ __forceinline__ double block_sum(double x) {
   return s;
 }
 
-// squares are formed and added in fp64 (a large fp32 gradient's square leaves fp32's range), in an order that depends on
-// the sizes alone: per thread, per block, then grad_norm_final over the blocks
-__global__ __launch_bounds__(kThreads) void grad_norm_kernel(GradLaunch a, double* __restrict__ part) {
-  double acc = 0.0;
-  for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-    const GradSlot& s = a.s[find_slot(a, c)];
-    const int64_t base = (int64_t)(c - s.first) * kGradChunk + (int64_t)threadIdx.x * 4;
-    const int type = s.type;
-    f4 x[4];
+// one chunk in registers: vectors of 16 bytes, what lies at n and beyond is zero
+struct Chunk32 {
+  f4 x[4];
+  __device__ __forceinline__ void load(const void* g, int64_t base, int64_t n) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = load4(s.g, type, base + u * kThreads * 4, s.n);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc = fma((double)x[u][j], (double)x[u][j], acc);
+    for (int u = 0; u < 4; ++u) x[u] = load4(g, OIVAE_F32, base + (u * kThreads + threadIdx.x) * 4, n);
   }
-  acc = block_sum(acc);
-  if (threadIdx.x == 0) part[blockIdx.x] = acc;
-}
-
-struct Advance {
-  int32_t which[kAdvance];
-  int32_t count;
+};
+typedef uint16_t h8 __attribute__((ext_vector_type(8)));
+typedef uint16_t h8u __attribute__((ext_vector_type(8), aligned(2)));
+struct Chunk16 {
+  h8 x[4];
+  __device__ __forceinline__ void load(const void* g, int64_t base, int64_t n) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t i = base + (u * kThreads + threadIdx.x) * 8;
+      const uint16_t* q = static_cast<const uint16_t*>(g) + i;
+      x[u] = h8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (i + 8 <= n) {
+        x[u] = *reinterpret_cast<const h8u*>(q);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 7; ++j)
+          if (i + j < n) x[u][j] = q[j];
+      }
+    }
+  }
 };
 
-// One block: the norm, the coefficient, whether the step is to be left out (a norm that is not finite, or a failed launch
-// behind the gradients: common.h ErrWords), and -- unless it is -- the step counters of the tensors that take part.
-// `parts` < 0: the verdict in `clip` stands already (further counters of the same step).
-__global__ __launch_bounds__(kThreads) void grad_norm_final(const double* __restrict__ part, int parts, float grad_scale,
-                                                            float max_norm, oivae_clip_t* clip, int32_t* steps, Advance adv,
-                                                            const uint32_t* __restrict__ bad) {
+// Squares are formed and added in fp64 -- a large gradient's square leaves fp32's range -- in an order that depends on the
+// sizes alone: per thread, per block, then over the blocks.
+__device__ __forceinline__ double sum_of_squares(const GradLaunch& a) {
+  double acc[2] = {0.0, 0.0};
+  for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
+    const GradSlot& s = a.s[find_slot(a, c)];
+    const int type = s.info & 3;
+    const int64_t base = (int64_t)(c - s.first) * grad_chunk(type);
+    if (type == OIVAE_F32) {
+      Chunk32 k;
+      k.load(s.g, base, s.n);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j & 1] = fma((double)k.x[u][j], (double)k.x[u][j], acc[j & 1]);
+    } else {
+      Chunk16 k;
+      k.load(s.g, base, s.n);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const double x = (double)half_to_float(k.x[u][j], type);
+          acc[j & 1] = fma(x, x, acc[j & 1]);
+        }
+    }
+  }
+  return block_sum(acc[0] + acc[1]);
+}
+
+__device__ __forceinline__ float clip_coef(float norm, float max_norm) {
+  const float limit = max_norm > 0.f ? max_norm / (norm + 1e-6f) : 1.f;
+  return limit > 1.f ? 1.f : limit;   // NaN stays
+}
+
+struct Verdict {
+  float grad_scale, max_norm;
+  oivae_clip_t* clip;
+  oivae_step_t* steps;
+  double ln_b1, ln_b2;
+  const uint32_t* bad;
+};
+
+// One block's work: the norm, the coefficient, whether the step is to be left out (a norm that is not finite, or a failed
+// launch behind the gradients: common.h ErrWords), and -- unless it is -- the step counters of the launch's tensors, with
+// their bias corrections.  `parts` < 0: the verdict stands already (further tensors of the same step).
+__device__ __forceinline__ void conclude(const GradLaunch& a, const double* part, int parts, const Verdict& v) {
   int skip;
   if (parts >= 0) {
     double s = 0.0;
-    for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
-    s = block_sum(s);
-    const float norm = (float)(sqrt(s) * fabs((double)grad_scale));
-    const float limit = max_norm > 0.f ? max_norm / (norm + 1e-6f) : 1.f;
-    skip = (bad != nullptr && *bad != 0) || !(fabsf(norm) <= 3.402823466e38f);
+    for (int i = threadIdx.x; i < parts; i += kThreads) s += __hip_atomic_load(part + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const float norm = (float)(sqrt(block_sum(s)) * fabs((double)v.grad_scale));
+    skip = (v.bad != nullptr && *v.bad != 0) || !(fabsf(norm) <= 3.402823466e38f);
     if (threadIdx.x == 0) {
-      clip->norm = norm;
-      clip->coef = limit > 1.f ? 1.f : limit;   // NaN stays
-      clip->skip = skip;
-      if (steps != nullptr) clip->skipped += skip;
+      v.clip->norm = norm;
+      v.clip->coef = clip_coef(norm, v.max_norm);
+      v.clip->skip = skip;
+      if (v.steps != nullptr) v.clip->skipped += skip;
     }
   } else {
-    skip = clip->skip;
+    skip = v.clip->skip;
   }
-  if (steps == nullptr || skip) return;
-  for (int i = threadIdx.x; i < adv.count; i += kThreads) steps[adv.which[i]] += 1;
+  if (v.steps == nullptr || skip) return;
+  for (int i = threadIdx.x; i < a.count; i += kThreads) {
+    const uint32_t index = a.s[i].info >> 2;
+    if (index == 0) continue;
+    oivae_step_t& q = v.steps[index - 1];
+    const int t = q.t + 1;
+    q.t = t;
+    // 1 - b^t = -expm1(t ln b) keeps its digits where b^t is near 1 (t = 1, b2 = 0.999)
+    q.inv_bc1 = (float)(1.0 / -expm1(t * v.ln_b1));
+    q.inv_bc2_sqrt = (float)(1.0 / sqrt(-expm1(t * v.ln_b2)));
+  }
 }
 
-__global__ __launch_bounds__(kThreads) void grad_clip_kernel(GradLaunch a, const oivae_clip_t* __restrict__ clip) {
-  const float coef = clip->coef;
-  if (coef == 1.f) return;   // nothing to scale
+__global__ __launch_bounds__(kThreads) void grad_norm_kernel(GradLaunch a, double* __restrict__ part) {
+  const double s = sum_of_squares(a);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(kThreads) void grad_norm_final(GradLaunch a, const double* __restrict__ part, int parts, Verdict v) {
+  conclude(a, part, parts, v);
+}
+
+// Both in one launch, the last block to arrive concluding; clip->ticket is zero before and after.  For few blocks: their
+// arrivals at one word take about 14 ns each, one after the other, a second launch about 4 us.
+__global__ __launch_bounds__(kThreads) void grad_norm_one(GradLaunch a, double* part, Verdict v) {
+  __shared__ int last;
+  const double s = sum_of_squares(a);
+  if (threadIdx.x == 0) {
+    __hip_atomic_store(part + blockIdx.x, s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t k = __hip_atomic_fetch_add(&v.clip->ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    last = k == gridDim.x - 1;
+    if (last) __hip_atomic_store(&v.clip->ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (last) conclude(a, part, (int)gridDim.x, v);
+}
+
+__global__ __launch_bounds__(kThreads) void norm_kernel(const double* __restrict__ part, int parts, float* norm) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
+  s = block_sum(s);
+  if (threadIdx.x == 0) *norm = (float)sqrt(s);
+}
+
+// g *= coef.  With parts > 0 every block adds the partial sums itself (few of them: cheaper than a launch between), and the
+// first one of the first launch leaves the norm.
+__global__ __launch_bounds__(kThreads) void grad_clip_kernel(GradLaunch a, const double* __restrict__ part, int parts, float max_norm,
+                                                             float* norm_out, int first) {
+  float norm;
+  if (parts > 0) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < parts; i += kThreads) s += part[i];
+    norm = (float)sqrt(block_sum(s));
+    if (first && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  } else {
+    norm = *norm_out;
+  }
+  const float coef = clip_coef(norm, max_norm);
+  if (coef == 1.f) return;   // a product with one
   for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
     const GradSlot& s = a.s[find_slot(a, c)];
-    const int64_t base = (int64_t)(c - s.first) * kGradChunk + (int64_t)threadIdx.x * 4;
-    const int type = s.type;
-    f4 x[4];
+    const int type = s.info & 3;
+    const int64_t base = (int64_t)(c - s.first) * grad_chunk(type), n = s.n;
+    if (type == OIVAE_F32) {
+      Chunk32 k;
+      k.load(s.g, base, n);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = load4(s.g, type, base + u * kThreads * 4, s.n);
+      for (int u = 0; u < 4; ++u) {
+        const int64_t i = base + (u * kThreads + threadIdx.x) * 4;
+        if (i < n) store4(s.g, OIVAE_F32, i, n, k.x[u] * coef);
+      }
+    } else {
+      Chunk16 k;
+      k.load(s.g, base, n);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (base + u * kThreads * 4 < s.n) store4(s.g, type, base + u * kThreads * 4, s.n, x[u] * coef);
+      for (int u = 0; u < 4; ++u) {
+        const int64_t i = base + (u * kThreads + threadIdx.x) * 8;
+        uint16_t* q = static_cast<uint16_t*>(s.g) + i;
+        h8 y;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = float_to_half(half_to_float(k.x[u][j], type) * coef, type);
+        if (i + 8 <= n) {
+          *reinterpret_cast<h8u*>(q) = y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 7; ++j)
+            if (i + j < n) q[j] = y[j];
+        }
+      }
+    }
   }
 }
 
@@ -212,87 +357,102 @@ struct AdamwSlot {
   int64_t n;
   uint32_t at;      // its first moment block in the flat moment buffers
   uint32_t first;   // its first chunk in the launch
-  uint32_t key;     // its index: of its step counter, and of its random bits
-  int32_t step;     // t, where no counters on the device are given
+  uint32_t index;   // of its step counter, and of its random bits
   int32_t types;    // gradient | parameter << 8
-  int32_t group;
+  int32_t option;   // index into the launch's Options
+  int32_t pad;
+};
+struct Options {
+  float lr, weight_decay;
+  const float* lr_dev;
+  float inv_bc1, inv_bc2_sqrt;
+  int32_t step;     // t and its corrections, where no counters on the device are given
+  int32_t pad;
 };
 struct AdamwLaunch {
   AdamwSlot s[kSlots];
-  oivae_adamw_group_t grp[kGroups];
+  Options opt[kOptions];
   oivae_adamw_state_t st;
   const oivae_clip_t* clip;
   const uint32_t* bad;
-  float ln_b1, ln_b2, b1, omb1, b2, omb2, eps, gscale;
+  float b1, omb1, b2, omb2, eps, gscale;
   uint32_t seed;
   int32_t count;
 };
 static_assert(sizeof(AdamwLaunch) <= 4096 && sizeof(GradLaunch) <= 4096, "kernel arguments of 4 KiB at most");
-constexpr int kChunk = 4096;   // elements of one workgroup
 
-struct StepScalars {
+// What a workgroup needs of its tensor; everything uniform.  The two words that can call the step off are read here and
+// looked at before the stores, so that the tensor's loads do not wait for them.
+struct Tile {
+  const void* g;
+  void* p;
+  int64_t n, flat, base;   // size; place in the moment buffers; the workgroup's first element
+  uint32_t at, index, step, off;
+  int gt, pt;
   float gscale, decay, step_size, inv_bc2_sqrt;
 };
 
-// bias corrections from t itself: 1 - b^t = -expm1(t ln b) keeps its digits where b^t is near 1 (t = 1, b2 = 0.999)
-__device__ __forceinline__ StepScalars step_scalars(const AdamwLaunch& a, const AdamwSlot& s) {
-  const float t = (float)(a.st.steps != nullptr ? a.st.steps[s.key] : s.step);
-  const oivae_adamw_group_t& q = a.grp[s.group];
-  const float lr = q.lr_dev != nullptr ? *q.lr_dev : q.lr;
-  StepScalars r;
-  r.gscale = a.clip != nullptr ? a.gscale * a.clip->coef : a.gscale;
+// a word behind a pointer of the argument struct, by a global load (the compiler takes such a pointer for a generic one)
+template <class T>
+__device__ __forceinline__ T word(const T* p) {
+  return *(const __attribute__((address_space(1))) T*)p;
+}
+
+__device__ __forceinline__ Tile find_tile(const AdamwLaunch& a) {
+  const AdamwSlot& s = a.s[find_slot(a, blockIdx.x)];
+  const Options& q = a.opt[s.option];
+  Tile r;
+  r.off = (a.bad != nullptr ? word(a.bad) : 0u) | (a.clip != nullptr ? (uint32_t)word(&a.clip->skip) : 0u);
+  r.g = s.g;
+  r.p = s.p;
+  r.n = s.n;
+  r.at = s.at;
+  r.flat = (int64_t)s.at * kMomentBlock;
+  r.base = (int64_t)(blockIdx.x - s.first) * kChunk;
+  r.index = s.index;
+  r.gt = s.types & 255;
+  r.pt = s.types >> 8;
+  float inv_bc1 = q.inv_bc1;
+  r.inv_bc2_sqrt = q.inv_bc2_sqrt;
+  r.step = (uint32_t)q.step;
+  if (a.st.steps != nullptr) {
+    const oivae_step_t* t = a.st.steps + s.index;
+    inv_bc1 = word(&t->inv_bc1);
+    r.inv_bc2_sqrt = word(&t->inv_bc2_sqrt);
+    r.step = (uint32_t)word(&t->t);
+  }
+  const float lr = q.lr_dev != nullptr ? word(q.lr_dev) : q.lr;
+  r.gscale = a.clip != nullptr ? a.gscale * word(&a.clip->coef) : a.gscale;
   r.decay = 1.f - lr * q.weight_decay;
-  r.step_size = lr / -expm1f(t * a.ln_b1);
-  r.inv_bc2_sqrt = 1.f / sqrtf(-expm1f(t * a.ln_b2));
+  r.step_size = lr * inv_bc1;
   return r;
 }
 
-__device__ __forceinline__ bool left_out(const AdamwLaunch& a) {
-  return (a.bad != nullptr && *a.bad != 0) || (a.clip != nullptr && a.clip->skip != 0);
-}
-
+// One vector of four elements per thread and stream: the loads of a wave are 1 KiB pieces, and a small workgroup keeps its
+// four streams short, so that many are in flight.  1024 elements a workgroup against 2048 / 4096 on 268M bf16 parameters:
+// 1279 against 1364 / 1332 us; with weights and moments through the caches 1420 us.
 __global__ __launch_bounds__(kThreads) void adamw32_kernel(AdamwLaunch a) {
-  if (left_out(a)) return;
-  const AdamwSlot& s = a.s[find_slot(a, blockIdx.x)];
-  const StepScalars r = step_scalars(a, s);
-  const int gt = s.types & 255, pt = s.types >> 8;
-  const int64_t n = s.n, flat = (int64_t)s.at * kMomentBlock;
-  float* __restrict__ m = static_cast<float*>(a.st.m) + flat;
-  float* __restrict__ v = static_cast<float*>(a.st.v) + flat;
-  float* __restrict__ w = pt == OIVAE_F32 ? static_cast<float*>(s.p) : a.st.master + flat;
-  const int64_t base = (int64_t)(blockIdx.x - s.first) * kChunk + (int64_t)threadIdx.x * 4;
-  f4 gi[4], wi[4], mi[4], vi[4];
+  const Tile r = find_tile(a);
+  const int64_t i = r.base + threadIdx.x * 4;
+  if (i >= r.n) return;
+  float* __restrict__ m = static_cast<float*>(a.st.m) + r.flat + i;   // moments occupy whole blocks: a vector that begins
+  float* __restrict__ v = static_cast<float*>(a.st.v) + r.flat + i;   // inside the tensor ends inside its block
+  float* __restrict__ w = r.pt == OIVAE_F32 ? static_cast<float*>(r.p) : a.st.master + r.flat;
+  const f4 gi = load4(r.g, r.gt, i, r.n);
+  f4 wi = stream4(w, i, r.n);
+  f4 mi = __builtin_nontemporal_load(reinterpret_cast<const f4*>(m)), vi = __builtin_nontemporal_load(reinterpret_cast<const f4*>(v));
+  if (r.off) return;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t i = base + u * kThreads * 4;
-    gi[u] = load4(s.g, gt, i, n);
-    wi[u] = load4(w, OIVAE_F32, i, n);
-    mi[u] = f4{0.f, 0.f, 0.f, 0.f};
-    vi[u] = f4{0.f, 0.f, 0.f, 0.f};
-    if (i < n) {   // moments occupy whole blocks: a vector that begins inside the tensor ends inside its block
-      mi[u] = *reinterpret_cast<const f4*>(m + i);
-      vi[u] = *reinterpret_cast<const f4*>(v + i);
-    }
+  for (int j = 0; j < 4; ++j) {
+    const float g = gi[j] * r.gscale;
+    mi[j] = fmaf(a.omb1, g, a.b1 * mi[j]);
+    vi[j] = fmaf(a.omb2 * g, g, a.b2 * vi[j]);
+    wi[j] = fmaf(-r.step_size, mi[j] / fmaf(sqrtf(vi[j]), r.inv_bc2_sqrt, a.eps), wi[j] * r.decay);
   }
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int64_t i = base + u * kThreads * 4;
-    if (i >= n) break;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float g = gi[u][j] * r.gscale;
-      const float mj = fmaf(a.omb1, g, a.b1 * mi[u][j]);
-      const float vj = fmaf(a.omb2 * g, g, a.b2 * vi[u][j]);
-      const float d = fmaf(sqrtf(vj), r.inv_bc2_sqrt, a.eps);
-      wi[u][j] = fmaf(-r.step_size, mj / d, wi[u][j] * r.decay);
-      mi[u][j] = mj;
-      vi[u][j] = vj;
-    }
-    *reinterpret_cast<f4*>(m + i) = mi[u];
-    *reinterpret_cast<f4*>(v + i) = vi[u];
-    store4(w, OIVAE_F32, i, n, wi[u]);
-    if (pt != OIVAE_F32) store4(s.p, pt, i, n, wi[u]);
-  }
+  __builtin_nontemporal_store(mi, reinterpret_cast<f4*>(m));
+  __builtin_nontemporal_store(vi, reinterpret_cast<f4*>(v));
+  stream4(w, i, r.n, wi);
+  if (r.pt != OIVAE_F32) stream4_half(r.p, r.pt, i, r.n, wi);
 }
 
 // ---- moments of 8 bits ----
@@ -303,8 +463,8 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(AdamwLaunch a) {
 // off, its expectation moves as it should.  A v that is not zero keeps at least the smallest code, so that an element never
 // divides a live first moment by eps alone.
 //   The power of two brings the block's largest magnitude into [2^7, 2^8) (e4m3's largest is 448) or [2^14, 2^15) (57344),
-// so rounding up never leaves the format; and a second exact scaling puts the code's subnormal spacing on fp32's own, where
-// code = (fp32 bits + random bits) >> 20 or 21, subnormal codes included.
+// so rounding up never leaves the format.  v_cvt_sr_fp8_f32 / v_cvt_sr_bf8_f32 add the upper 20 or 21 of 32 random bits
+// below the code's last place and cut off, subnormal codes included.
 constexpr uint32_t kMix1 = 0x9E3779B1u, kMix2 = 0x6A09E667u, kMix3 = 0xBB67AE85u, kMix4 = 0x3C6EF373u;   // 2^32 times the
 // fractions of the golden ratio and of the roots of 2, 3 and 5, made odd
 
@@ -324,105 +484,94 @@ __device__ __forceinline__ uint32_t max16(uint32_t x) {
   return x;
 }
 
+// ... of 32
+__device__ __forceinline__ uint32_t max32(uint32_t x) {
+  x = max16(x);
+  const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);   // rows 0, 0, 2, 2 and rows 1, 1, 3, 3
+  return max((uint32_t)p[0], (uint32_t)p[1]);
+}
+
 __device__ __forceinline__ float scale_of(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float(byte << 23);
 }
 
-__device__ __forceinline__ uint32_t pack_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return (a & 255u) | (b & 255u) << 8 | (c & 255u) << 16 | d << 24;
-}
-
-// 16 lanes hold one block, 8 elements each
+// 32 lanes hold one block, four elements each (one vector per thread and stream, as above).  With 16 lanes and 8 elements
+// a lane the vectors of a wave are 32 bytes apart: 861 us on 268M bf16 parameters against 719.
+//   kFast: hardware root and reciprocal (one unit in the last place each) instead of the correctly rounded ones, 45 of 120
+// instructions an element: 719 against 779 us.  The hardware root takes subnormals for zero, an error of 1.1e-19 in the
+// root and of 3.5e-18 in the denominator (t = 1, b2 = 0.999), below its last place while eps >= 1e-10.
+template <bool kFast>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(AdamwLaunch a) {
-  if (left_out(a)) return;
-  const AdamwSlot& s = a.s[find_slot(a, blockIdx.x)];
-  const StepScalars r = step_scalars(a, s);
-  const int gt = s.types & 255, pt = s.types >> 8;
-  const int64_t n = s.n, flat = (int64_t)s.at * kMomentBlock;
-  uint8_t* __restrict__ m = static_cast<uint8_t*>(a.st.m) + flat;
-  uint8_t* __restrict__ v = static_cast<uint8_t*>(a.st.v) + flat;
-  uint8_t* __restrict__ ms = a.st.m_scale + s.at;
-  uint8_t* __restrict__ vs = a.st.v_scale + s.at;
-  float* __restrict__ w = pt == OIVAE_F32 ? static_cast<float*>(s.p) : a.st.master + flat;
-  const uint32_t key = random_key(a.seed, (uint32_t)(a.st.steps != nullptr ? a.st.steps[s.key] : s.step), s.key);
-  const int64_t end = (n + kMomentBlock - 1) / kMomentBlock * kMomentBlock;
-#pragma unroll 1
-  for (int u = 0; u < kChunk / (kThreads * 8); ++u) {
-    const int64_t i = (int64_t)(blockIdx.x - s.first) * kChunk + u * kThreads * 8 + (int64_t)threadIdx.x * 8;
-    if (i >= end) break;   // whole blocks, that is whole rows of 16 lanes, leave together
-    const int64_t blk = i / kMomentBlock;
-    const f4 g0 = load4(s.g, gt, i, n), g1 = load4(s.g, gt, i + 4, n);
-    f4 w0 = load4(w, OIVAE_F32, i, n), w1 = load4(w, OIVAE_F32, i + 4, n);
-    const u2 mc = *reinterpret_cast<const u2*>(m + i), vc = *reinterpret_cast<const u2*>(v + i);
-    const float msc = scale_of(ms[blk]), vsc = scale_of(vs[blk]);
-    float g[8], wj[8], mj[8], vj[8];
+  const Tile r = find_tile(a);
+  const int64_t i = r.base + threadIdx.x * 4;
+  const int64_t blk = i / kMomentBlock;
+  if (blk >= (r.n + kMomentBlock - 1) / kMomentBlock) return;   // whole blocks, that is whole halves of a wave, leave together
+  uint32_t* __restrict__ m = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.st.m) + r.flat + i);
+  uint32_t* __restrict__ v = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.st.v) + r.flat + i);
+  uint8_t* __restrict__ ms = a.st.m_scale + r.at + blk;
+  uint8_t* __restrict__ vs = a.st.v_scale + r.at + blk;
+  float* __restrict__ w = r.pt == OIVAE_F32 ? static_cast<float*>(r.p) : a.st.master + r.flat;
+  const f4 gi = load4(r.g, r.gt, i, r.n);
+  f4 wi = stream4(w, i, r.n);
+  const int mc = (int)*m, vc = (int)*v;
+  const float msc = scale_of(*ms), vsc = scale_of(*vs);
+  if (r.off) return;
+  const f2v m0 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, true);
+  const f2v v0 = __builtin_amdgcn_cvt_pk_f32_bf8(vc, false), v1 = __builtin_amdgcn_cvt_pk_f32_bf8(vc, true);
+  float mj[4] = {m0[0], m0[1], m1[0], m1[1]}, vj[4] = {v0[0], v0[1], v1[0], v1[1]};
+  uint32_t mmax = 0, vmax = 0;   // magnitudes as bit patterns: a NaN is larger than everything and stays visible
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      g[j] = g0[j] * r.gscale; g[4 + j] = g1[j] * r.gscale;
-      wj[j] = w0[j]; wj[4 + j] = w1[j];
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f2v ml = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[h], false), mh = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[h], true);
-      const f2v vl = __builtin_amdgcn_cvt_pk_f32_bf8((int)vc[h], false), vh = __builtin_amdgcn_cvt_pk_f32_bf8((int)vc[h], true);
-      mj[4 * h] = ml[0]; mj[4 * h + 1] = ml[1]; mj[4 * h + 2] = mh[0]; mj[4 * h + 3] = mh[1];
-      vj[4 * h] = vl[0]; vj[4 * h + 1] = vl[1]; vj[4 * h + 2] = vh[0]; vj[4 * h + 3] = vh[1];
-    }
-    uint32_t mmax = 0, vmax = 0;   // magnitudes as bit patterns: a NaN is larger than everything and stays visible
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      mj[j] = (mj[j] * msc) * a.b1 + g[j] * a.omb1;
-      vj[j] = (vj[j] * vsc) * a.b2 + (g[j] * g[j]) * a.omb2;
-      const float d = sqrtf(vj[j]) * r.inv_bc2_sqrt + a.eps;
-      wj[j] = wj[j] * r.decay - r.step_size * (mj[j] / d);
-      mmax = max(mmax, __float_as_uint(mj[j]) & 0x7FFFFFFFu);
-      vmax = max(vmax, __float_as_uint(vj[j]) & 0x7FFFFFFFu);
-    }
-    const uint32_t me = max16(mmax) >> 23, ve = max16(vmax) >> 23;
-    const uint32_t mb = me == 255u ? 255u : max(me, 8u) - 7u, vb = ve == 255u ? 255u : max(ve, 15u) - 14u;
-    const int mshift = 127 - (int)mb - 120, vshift = 127 - (int)vb - 112;
-    const uint64_t e0 = (uint64_t)i;
-    const uint32_t x0 = (uint32_t)e0 * kMix1 + (uint32_t)(e0 >> 32) * kMix4 + key;
-    uint32_t mq[8], vq[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t x = x0 + (uint32_t)j * kMix1;
-      x = (x ^ (x >> 14)) * kMix2;
-      x ^= x >> 14;
-      const uint32_t zm = __float_as_uint(__builtin_amdgcn_ldexpf(mj[j], mshift));
-      const uint32_t zv = __float_as_uint(__builtin_amdgcn_ldexpf(vj[j], vshift));
-      mq[j] = ((zm & 0x7FFFFFFFu) + (x >> 12)) >> 20 | (zm >> 31) << 7;
-      vq[j] = max((zv + (x & 0x1FFFFFu)) >> 21, vj[j] > 0.f ? 1u : 0u);
-    }
-    const u2 mo = {pack_bytes(mq[0], mq[1], mq[2], mq[3]), pack_bytes(mq[4], mq[5], mq[6], mq[7])};
-    const u2 vo = {pack_bytes(vq[0], vq[1], vq[2], vq[3]), pack_bytes(vq[4], vq[5], vq[6], vq[7])};
-    *reinterpret_cast<u2*>(m + i) = mo;
-    *reinterpret_cast<u2*>(v + i) = vo;
-    if ((threadIdx.x & 15) == 0) {
-      ms[blk] = (uint8_t)mb;
-      vs[blk] = (uint8_t)vb;
-    }
-    w0 = f4{wj[0], wj[1], wj[2], wj[3]};
-    w1 = f4{wj[4], wj[5], wj[6], wj[7]};
-    if (i < n) store4(w, OIVAE_F32, i, n, w0);
-    if (i + 4 < n) store4(w, OIVAE_F32, i + 4, n, w1);
-    if (pt != OIVAE_F32) {
-      if (i < n) store4(s.p, pt, i, n, w0);
-      if (i + 4 < n) store4(s.p, pt, i + 4, n, w1);
-    }
+  for (int j = 0; j < 4; ++j) {
+    const float g = gi[j] * r.gscale;
+    mj[j] = (mj[j] * msc) * a.b1 + g * a.omb1;
+    vj[j] = (vj[j] * vsc) * a.b2 + (g * g) * a.omb2;
+    const float q = kFast ? mj[j] * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(vj[j]), r.inv_bc2_sqrt, a.eps))
+                          : mj[j] / fmaf(sqrtf(vj[j]), r.inv_bc2_sqrt, a.eps);
+    wi[j] = fmaf(-r.step_size, q, wi[j] * r.decay);
+    mmax = max(mmax, __float_as_uint(mj[j]) & 0x7FFFFFFFu);
+    vmax = max(vmax, __float_as_uint(vj[j]));
   }
+  const uint32_t me = max32(mmax) >> 23, ve = max32(vmax) >> 23;
+  const uint32_t mb = me == 255u ? 255u : max(me, 8u) - 7u, vb = ve == 255u ? 255u : max(ve, 15u) - 14u;
+  const uint32_t x0 = (uint32_t)i * kMix1 + (uint32_t)((uint64_t)i >> 32) * kMix4 + random_key(a.seed, r.step, r.index);
+  int mq = 0, vq = 0;
+  auto one = [&](auto J) {
+    constexpr int j = decltype(J)::value;
+    uint32_t x = x0 + (uint32_t)j * kMix1;
+    x = (x ^ (x >> 14)) * kMix2;
+    x ^= x >> 14;
+    const float zm = __builtin_amdgcn_ldexpf(mj[j], 127 - (int)mb), zv = __builtin_amdgcn_ldexpf(vj[j], 127 - (int)vb);
+    mq = __builtin_amdgcn_cvt_sr_fp8_f32(zm, (int)x, mq, j);
+    vq = __builtin_amdgcn_cvt_sr_bf8_f32(vj[j] > 0.f ? fmaxf(zv, 0x1p-16f) : 0.f, (int)(x << 11), vq, j);
+  };
+  one(std::integral_constant<int, 0>{});
+  one(std::integral_constant<int, 1>{});
+  one(std::integral_constant<int, 2>{});
+  one(std::integral_constant<int, 3>{});
+  *m = (uint32_t)mq;
+  *v = (uint32_t)vq;
+  if ((threadIdx.x & 31) == 0) {
+    *ms = (uint8_t)mb;
+    *vs = (uint8_t)vb;
+  }
+  if (i >= r.n) return;
+  stream4(w, i, r.n, wi);
+  if (r.pt != OIVAE_F32) stream4_half(r.p, r.pt, i, r.n, wi);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 static bool aligned_to(const void* p, int a) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(a - 1)) == 0; }
 static int size_of(int type) { return type == OIVAE_F32 ? 4 : 2; }
 
+constexpr uint32_t kMaxChunks = 0xFFFFFFu;   // workgroups of one launch: a grid's size in threads stays below 2^32
+constexpr int64_t kMaxElements = (int64_t)kMaxChunks * kChunk;   // of one tensor
+
 static int check_grad(const char* who, int32_t i, const void* g, int64_t n, int32_t type) {
   if (n < 0) return fail(OIVAE_E_ARG, "%s: tensor %d has a negative size", who, i);
   if (type < OIVAE_F32 || type > OIVAE_F16) return fail(OIVAE_E_ARG, "%s: tensor %d has unknown gradient type %d", who, i, type);
   if (n > 0 && !g) return fail(OIVAE_E_ARG, "%s: tensor %d has a null gradient", who, i);
   if (!aligned_to(g, size_of(type))) return fail(OIVAE_E_ARG, "%s: gradient %d is not aligned to its elements", who, i);
-  if (n > (int64_t)1 << 40) return fail(OIVAE_E_SHAPE, "%s: tensor %d has more than 2^40 elements", who, i);
+  if (n > kMaxElements) return fail(OIVAE_E_SHAPE, "%s: tensor %d has more than %lld elements", who, i, (long long)kMaxElements);
   return OIVAE_OK;
 }
 
@@ -433,17 +582,42 @@ static int for_grad_launches(const oivae_grad_t* t, int32_t count, F&& launch) {
   a.count = 0;
   a.chunks = 0;
   for (int32_t i = 0; i < count; ++i) {
-    if (t[i].n == 0) continue;
-    const uint32_t c = (uint32_t)((t[i].n + kGradChunk - 1) / kGradChunk);
+    if (t[i].n == 0 && t[i].index < 0) continue;
+    const int ck = grad_chunk(t[i].type);
+    const uint32_t c = (uint32_t)((t[i].n + ck - 1) / ck);
     if (a.count == kGradSlots || (a.count > 0 && a.chunks + (uint64_t)c > (1u << 30))) {
       if (int rc = launch(a)) return rc;
       a.count = 0;
       a.chunks = 0;
     }
-    a.s[a.count++] = GradSlot{t[i].g, t[i].n, a.chunks, t[i].type};
+    a.s[a.count++] = GradSlot{t[i].g, t[i].n, a.chunks, (uint32_t)t[i].type | (uint32_t)(t[i].index + 1) << 2};
     a.chunks += c;
   }
   return a.count > 0 ? launch(a) : OIVAE_OK;
+}
+
+static int check_grads(const char* who, const oivae_grad_t* t, int32_t count, void* workspace, int64_t workspace_bytes) {
+  for (int32_t i = 0; i < count; ++i) {
+    if (int rc = check_grad(who, i, t[i].g, t[i].n, t[i].type)) return rc;
+    if (t[i].index < -1 || t[i].index >= 1 << 29) return fail(OIVAE_E_ARG, "%s: tensor %d has index %d", who, i, t[i].index);
+  }
+  if (!workspace || !aligned_to(workspace, 8) || workspace_bytes < oivae_grad_norm_workspace_bytes(count))
+    return fail(OIVAE_E_WORKSPACE, "%s: workspace of %lld bytes (8-byte aligned) needed", who,
+                (long long)oivae_grad_norm_workspace_bytes(count));
+  return OIVAE_OK;
+}
+
+// the partial sums of all launches, one behind the other; their number into `parts`
+static int launch_partials(const oivae_grad_t* t, int32_t count, double* part, int64_t* parts, hipStream_t st) {
+  *parts = 0;
+  return for_grad_launches(t, count, [&](const GradLaunch& a) -> int {
+    if (a.chunks == 0) return OIVAE_OK;
+    const unsigned blocks = a.chunks < (uint32_t)kNormBlocks ? a.chunks : (unsigned)kNormBlocks;
+    hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(kThreads), 0, st, a, part + *parts);
+    OIVAE_LAUNCH_CHECK();
+    *parts += blocks;
+    return OIVAE_OK;
+  });
 }
 
 static int run_adamw(const char* who, bool eight, const oivae_adamw_tensor_t* t, int32_t count, const oivae_adamw_group_t* groups,
@@ -474,19 +648,20 @@ static int run_adamw(const char* who, bool eight, const oivae_adamw_tensor_t* t,
   a.st = *st;
   a.clip = clip;
   a.bad = bad_word_device();
-  a.ln_b1 = (float)log(beta1); a.ln_b2 = (float)log(beta2);
   a.b1 = (float)beta1; a.omb1 = (float)(1.0 - beta1);   // the differences in double: 1 - 0.999f has lost five digits
   a.b2 = (float)beta2; a.omb2 = (float)(1.0 - beta2);
   a.eps = (float)eps;
   a.gscale = grad_scale;
   a.seed = seed;
-  int32_t names[kGroups], n_names = 0;
-  uint32_t chunks = 0;
   a.count = 0;
+  struct { int32_t group, step; } names[kOptions];
+  int32_t n_names = 0;
+  uint32_t chunks = 0;
   auto launch = [&]() -> int {
     if (a.count == 0) return OIVAE_OK;
-    if (eight) hipLaunchKernelGGL(adamw8_kernel, dim3(chunks), dim3(kThreads), 0, hs, a);
-    else hipLaunchKernelGGL(adamw32_kernel, dim3(chunks), dim3(kThreads), 0, hs, a);
+    if (!eight) hipLaunchKernelGGL(adamw32_kernel, dim3(chunks), dim3(kThreads), 0, hs, a);
+    else if (eps >= 1e-10) hipLaunchKernelGGL(adamw8_kernel<true>, dim3(chunks), dim3(kThreads), 0, hs, a);
+    else hipLaunchKernelGGL(adamw8_kernel<false>, dim3(chunks), dim3(kThreads), 0, hs, a);
     OIVAE_LAUNCH_CHECK();
     a.count = 0;
     n_names = 0;
@@ -495,22 +670,27 @@ static int run_adamw(const char* who, bool eight, const oivae_adamw_tensor_t* t,
   };
   for (int32_t i = 0; i < count; ++i) {
     if (t[i].n == 0) continue;
-    const uint32_t c = (uint32_t)((t[i].n + kChunk - 1) / kChunk);
+    const int32_t step = st->steps ? 0 : t[i].step;
+    const uint64_t c = ((uint64_t)t[i].n + kChunk - 1) / kChunk;
     int32_t q = 0;
-    while (q < n_names && names[q] != t[i].group) ++q;
-    // a grid's size in threads stays below 2^32
-    if (a.count == kSlots || q == kGroups || (a.count > 0 && chunks + (uint64_t)c > 0xFFFFFFu)) {
+    while (q < n_names && (names[q].group != t[i].group || names[q].step != step)) ++q;
+    if (a.count == kSlots || q == kOptions || (a.count > 0 && chunks + c > kMaxChunks)) {
       if (int rc = launch()) return rc;
       q = 0;
     }
-    if (c > 0xFFFFFFu) return fail(OIVAE_E_SHAPE, "%s: tensor %d has more than %lld elements", who, i, (long long)0xFFFFFF * kChunk);
     if (q == n_names) {
-      names[n_names++] = t[i].group;
-      a.grp[q] = groups[t[i].group];
+      names[n_names].group = t[i].group;
+      names[n_names++].step = step;
+      const oivae_adamw_group_t& g = groups[t[i].group];
+      Options& o = a.opt[q];
+      o.lr = g.lr; o.weight_decay = g.weight_decay; o.lr_dev = g.lr_dev;
+      o.step = step;
+      o.inv_bc1 = step ? (float)(1.0 / -expm1(step * log(beta1))) : 1.f;
+      o.inv_bc2_sqrt = step ? (float)(1.0 / sqrt(-expm1(step * log(beta2)))) : 1.f;
     }
-    a.s[a.count++] = AdamwSlot{t[i].p, t[i].g, t[i].n, (uint32_t)(t[i].at / kMomentBlock), chunks, (uint32_t)t[i].index, t[i].step,
-                               t[i].g_type | t[i].p_type << 8, q};
-    chunks += c;
+    a.s[a.count++] = AdamwSlot{t[i].p, t[i].g, t[i].n, (uint32_t)(t[i].at / kMomentBlock), chunks, (uint32_t)t[i].index,
+                               t[i].g_type | t[i].p_type << 8, q, 0};
+    chunks += (uint32_t)c;
   }
   return launch();
 }
@@ -519,62 +699,79 @@ static int run_adamw(const char* who, bool eight, const oivae_adamw_tensor_t* t,
 
 using namespace oivae;
 
+// a launch takes kGradSlots tensors (fewer only where they come to 2^30 chunks, 4 TiB: one more launch covers that)
 extern "C" int64_t oivae_grad_norm_workspace_bytes(int32_t count) {
-  const int64_t launches = count <= 0 ? 1 : count;   // a launch takes at least one tensor (at most kGradSlots)
-  return (int64_t)sizeof(double) * kNormBlocks * ((launches + kGradSlots - 1) / kGradSlots + 1);
+  return (int64_t)sizeof(double) * kNormBlocks * ((count <= 0 ? 0 : (count - 1) / kGradSlots) + 2);
 }
 
-extern "C" int oivae_grad_norm(const oivae_grad_t* grads, int32_t count, float grad_scale, float max_norm, oivae_clip_t* clip,
-                               int32_t* steps, const int32_t* which, int32_t n_which, void* workspace, int64_t workspace_bytes,
-                               void* stream) {
+extern "C" int oivae_grad_norm(const oivae_grad_t* grads, int32_t count, int32_t with_norm, float grad_scale, float max_norm,
+                               oivae_clip_t* clip, oivae_step_t* steps, double beta1, double beta2, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
   const char* who = "oivae_grad_norm";
-  if (count < 0 || (count > 0 && !grads) || !clip || n_which < 0 || (n_which > 0 && (!which || !steps)))
-    return fail(OIVAE_E_ARG, "%s: bad argument", who);
-  if (!workspace || !aligned_to(workspace, 8) || workspace_bytes < oivae_grad_norm_workspace_bytes(count))
-    return fail(OIVAE_E_WORKSPACE, "%s: workspace of %lld bytes (8-byte aligned) needed", who,
-                (long long)oivae_grad_norm_workspace_bytes(count));
-  for (int32_t i = 0; i < count; ++i)
-    if (int rc = check_grad(who, i, grads[i].g, grads[i].n, grads[i].type)) return rc;
-  for (int32_t i = 0; i < n_which; ++i)
-    if (which[i] < 0) return fail(OIVAE_E_ARG, "%s: negative step counter index", who);
+  if (count < 0 || (count > 0 && !grads) || !clip) return fail(OIVAE_E_ARG, "%s: bad argument", who);
+  if (steps && !(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0))
+    return fail(OIVAE_E_ARG, "%s: betas must be in [0, 1)", who);
+  if (int rc = check_grads(who, grads, count, workspace, workspace_bytes)) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (int rc = poll_error_word(who, st)) return rc;
   double* part = static_cast<double*>(workspace);
-  const int64_t room = workspace_bytes / (int64_t)sizeof(double);
+  const Verdict v{grad_scale, max_norm, clip, steps, steps ? log(beta1) : 0.0, steps ? log(beta2) : 0.0, bad_word_device()};
+  int launches = 0;
+  uint32_t chunks = 0;
+  for_grad_launches(grads, count, [&](const GradLaunch& a) -> int {
+    ++launches;
+    chunks = a.chunks;
+    return OIVAE_OK;
+  });
+  if (with_norm && launches == 1 && chunks > 0 && chunks <= (uint32_t)kFewBlocks)
+    return for_grad_launches(grads, count, [&](const GradLaunch& a) -> int {
+      hipLaunchKernelGGL(grad_norm_one, dim3(a.chunks), dim3(kThreads), 0, st, a, part, v);
+      OIVAE_LAUNCH_CHECK();
+      return OIVAE_OK;
+    });
   int64_t parts = 0;
-  if (int rc = for_grad_launches(grads, count, [&](const GradLaunch& a) -> int {
-        const unsigned blocks = a.chunks < (uint32_t)kNormBlocks ? a.chunks : (unsigned)kNormBlocks;
-        if (parts + blocks > room) return fail(OIVAE_E_WORKSPACE, "%s: workspace too small for tensors this large", who);
-        hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(kThreads), 0, st, a, part + parts);
-        OIVAE_LAUNCH_CHECK();
-        parts += blocks;
-        return OIVAE_OK;
-      }))
-    return rc;
-  int32_t done = 0;
-  do {
-    Advance adv;
-    adv.count = n_which - done < kAdvance ? n_which - done : kAdvance;
-    for (int32_t i = 0; i < adv.count; ++i) adv.which[i] = which[done + i];
-    hipLaunchKernelGGL(grad_norm_final, dim3(1), dim3(kThreads), 0, st, (const double*)part, done == 0 ? (int)parts : -1,
-                       grad_scale, max_norm, clip, steps, adv, bad_word_device());
+  if (with_norm)
+    if (int rc = launch_partials(grads, count, part, &parts, st)) return rc;
+  bool first = true;
+  auto conclude_launch = [&](const GradLaunch& a) -> int {
+    if (!first && !steps) return OIVAE_OK;
+    hipLaunchKernelGGL(grad_norm_final, dim3(1), dim3(kThreads), 0, st, a, (const double*)part, first ? (int)parts : -1, v);
     OIVAE_LAUNCH_CHECK();
-    done += adv.count;
-  } while (done < n_which);
-  return OIVAE_OK;
+    first = false;
+    return OIVAE_OK;
+  };
+  if (launches > 0) return for_grad_launches(grads, count, conclude_launch);
+  GradLaunch none;
+  none.count = 0;
+  none.chunks = 0;
+  return conclude_launch(none);
 }
 
-extern "C" int oivae_grad_clip(const oivae_grad_t* grads, int32_t count, const oivae_clip_t* clip, void* stream) {
-  const char* who = "oivae_grad_clip";
-  if (count < 0 || (count > 0 && !grads) || !clip) return fail(OIVAE_E_ARG, "%s: bad argument", who);
-  for (int32_t i = 0; i < count; ++i)
-    if (int rc = check_grad(who, i, grads[i].g, grads[i].n, grads[i].type)) return rc;
+extern "C" int oivae_clip_grad_norm(const oivae_grad_t* grads, int32_t count, float max_norm, float* norm, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  const char* who = "oivae_clip_grad_norm";
+  if (count < 0 || (count > 0 && !grads) || !norm) return fail(OIVAE_E_ARG, "%s: bad argument", who);
+  if (int rc = check_grads(who, grads, count, workspace, workspace_bytes)) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (int rc = poll_error_word(who, st)) return rc;
-  return for_grad_launches(grads, count, [&](const GradLaunch& a) -> int {
-    const unsigned blocks = a.chunks < 8192u ? a.chunks : 8192u;
-    hipLaunchKernelGGL(grad_clip_kernel, dim3(blocks), dim3(kThreads), 0, st, a, clip);
+  double* part = static_cast<double*>(workspace);
+  int64_t parts = 0;
+  if (int rc = launch_partials(grads, count, part, &parts, st)) return rc;
+  const bool scale = max_norm > 0.f && parts > 0;
+  const bool few = scale && parts <= kFewBlocks;
+  if (!few) {
+    hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, st, (const double*)part, (int)parts, norm);
     OIVAE_LAUNCH_CHECK();
+  }
+  if (!scale) return OIVAE_OK;
+  int first = 1;
+  return for_grad_launches(grads, count, [&](const GradLaunch& a) -> int {
+    if (a.chunks == 0) return OIVAE_OK;
+    const unsigned blocks = a.chunks < 8192u ? a.chunks : 8192u;
+    hipLaunchKernelGGL(grad_clip_kernel, dim3(blocks), dim3(kThreads), 0, st, a, (const double*)part, few ? (int)parts : 0, max_norm,
+                       norm, first);
+    OIVAE_LAUNCH_CHECK();
+    first = 0;
     return OIVAE_OK;
   });
 }

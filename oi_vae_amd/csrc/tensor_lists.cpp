@@ -48,7 +48,7 @@ struct Buffer {
 
 // parameters(list, records of oivae_adamw_tensor_t, device, records of oivae_grad_t or None) -> (first unusual tensor or -1,
 // number without a gradient).  Fills p, g and g_type, g = 0 where a parameter has no gradient, and the gradients' records
-// (n = 0 there).  The records' n and p_type say what the parameters have to be.
+// (n = 0 and index -1 there).  The records' n and p_type say what the parameters have to be.
 PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 4 || !PyList_Check(args[0])) {
     PyErr_SetString(PyExc_TypeError, "parameters(list, records, device, gradient records)");
@@ -73,7 +73,7 @@ PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       const at::Tensor& g = p.grad();
       if (!g.defined()) {
         r[i].g = nullptr;
-        if (q) q[i] = oivae_grad_t{nullptr, 0, OIVAE_F32, 0};
+        if (q) q[i] = oivae_grad_t{nullptr, 0, OIVAE_F32, -1};
         ++missing;
         unusual = -1;
         continue;
@@ -84,7 +84,7 @@ PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       r[i].p = p.data_ptr();
       r[i].g = g.data_ptr();
       r[i].g_type = type_of(g);
-      if (q) q[i] = oivae_grad_t{g.data_ptr(), g.numel(), type_of(g), 0};
+      if (q) q[i] = oivae_grad_t{g.data_ptr(), g.numel(), type_of(g), r[i].index};
       unusual = -1;
     }
   } catch (const std::exception& e) {
@@ -117,7 +117,7 @@ PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (!g.defined()) continue;
       if (device < 0 && g.is_cuda()) device = (int)g.get_device();
       if (!plain(g, device)) Py_RETURN_NONE;
-      r[count++] = oivae_grad_t{g.data_ptr(), g.numel(), type_of(g), 0};
+      r[count++] = oivae_grad_t{g.data_ptr(), g.numel(), type_of(g), -1};
       if (g.numel() > 0) seen.push_back(g.data_ptr());
     }
     std::sort(seen.begin(), seen.end());

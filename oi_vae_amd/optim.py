@@ -103,7 +103,7 @@ class SGD(_EngineOptimizer):
 
 # ---- lists of tensors ------------------------------------------------------------------------------------------------------
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
-_GRAD = np.dtype([("g", "u8"), ("n", "i8"), ("type", "i4"), ("pad", "i4")])                       # oivae_grad_t
+_GRAD = np.dtype([("g", "u8"), ("n", "i8"), ("type", "i4"), ("index", "i4")])                     # oivae_grad_t
 _TENSOR = np.dtype([("p", "u8"), ("g", "u8"), ("n", "i8"), ("at", "i8"), ("p_type", "i4"), ("g_type", "i4"),
                     ("group", "i4"), ("index", "i4"), ("step", "i4"), ("pad", "i4")])             # oivae_adamw_tensor_t
 _GROUP = np.dtype([("lr", "f4"), ("weight_decay", "f4"), ("lr_dev", "u8")])                       # oivae_adamw_group_t
@@ -170,20 +170,17 @@ def _grads_of(parameters):
   rec["g"] = [g.data_ptr() for g in packed]
   rec["n"] = [g.numel() for g in packed]
   rec["type"] = [_TYPES[g.dtype] for g in packed]
+  rec["index"] = -1
   return rec, device.index, grads, packed
 
 
-def _norm_of(rec, device, max_norm, scale):
+def _clip(rec, device, max_norm):
   L = _lib.init_device(device)
   nbytes = L.oivae_grad_norm_workspace_bytes(len(rec))
-  # verdict (16 bytes, written whole) and workspace of this call alone: calls on other streams and in captured graphs have
-  # their own
+  # norm and workspace of this call alone: calls on other streams and in captured graphs have their own
   ws = torch.empty(nbytes // 4 + 4, dtype=torch.float32, device=torch.device("cuda", device))
-  clip, address = ws.data_ptr(), rec.ctypes.data
-  stream = torch.cuda.current_stream(device).cuda_stream
-  _lib.check(L.oivae_grad_norm(address, len(rec), 1.0, max_norm, clip, None, None, 0, clip + 16, nbytes, stream), "oivae_grad_norm")
-  if scale:
-    _lib.check(L.oivae_grad_clip(address, len(rec), clip, stream), "oivae_grad_clip")
+  _lib.check(L.oivae_clip_grad_norm(rec.ctypes.data, len(rec), max_norm, ws.data_ptr(), ws.data_ptr() + 16, nbytes,
+                                    torch.cuda.current_stream(device).cuda_stream), "oivae_clip_grad_norm")
   return ws[0]
 
 
@@ -195,7 +192,7 @@ def grad_norm(parameters):
   if got is None:
     return torch.zeros(())
   with torch.cuda.device(got[1]):
-    return _norm_of(got[0], got[1], 0.0, False)
+    return _clip(got[0], got[1], 0.0)
 
 
 def clip_grad_norm_(parameters, max_norm):
@@ -209,7 +206,7 @@ def clip_grad_norm_(parameters, max_norm):
     return torch.zeros(())
   rec, device, grads, packed = got
   with torch.cuda.device(device):
-    norm = _norm_of(rec, device, max_norm, True)
+    norm = _clip(rec, device, max_norm)
     with torch.no_grad():
       for g, c in zip(grads, packed):
         if c is not g:
@@ -311,7 +308,7 @@ class AdamW(_EngineOptimizer):
     self._leaves, self.device = leaves, device
     self._lib = _lib.init_device(device.index)
     self._kinds = []
-    self._steps_dev = torch.zeros(len(leaves), dtype=torch.int32, device=device) if self._on_device else None
+    self._steps_dev = torch.zeros(len(leaves), 4, dtype=torch.int32, device=device) if self._on_device else None
     bits_of = [self.param_groups[g]["state_bits"] for g in groups]
     for bits in (32, 8):
       # 16-bit parameters first: the master buffer need not reach further than they do
@@ -319,12 +316,10 @@ class AdamW(_EngineOptimizer):
       if mine:
         self._kinds.append(_Kind(self, bits, mine, groups))
     buffers = {k.bits: k.held for k in self._kinds}
-    self._clip = torch.zeros(4, dtype=torch.int32, device=device) if self._on_device else None
+    self._clip = torch.zeros(8, dtype=torch.int32, device=device) if self._on_device else None
     if self._on_device:
       self._ws = torch.empty(self._lib.oivae_grad_norm_workspace_bytes(len(leaves)), dtype=torch.uint8, device=device)
-      # gradients' records and step counters of all kinds, one behind the other
-      self._norm_rec = np.zeros(len(leaves), _GRAD)
-      self._which = np.concatenate([k.rec["index"] for k in self._kinds]).astype(np.int32)
+      self._norm_rec = np.zeros(len(leaves), _GRAD)   # the gradients of all kinds, one behind the other
       at = 0
       for k in self._kinds:
         k.grads = self._norm_rec[at:at + len(k.mine)]
@@ -376,7 +371,7 @@ class AdamW(_EngineOptimizer):
     """Steps taken so far, parameter by parameter (a list; reads the device where the counts live there)."""
     self.buffers
     if self._on_device:
-      return self._steps_dev.tolist()
+      return self._steps_dev[:, 0].tolist()
     counts = np.zeros(len(self._leaves), np.int32)
     for k in self._kinds:
       counts[k.mine] = k.rec["step"]
@@ -391,7 +386,7 @@ class AdamW(_EngineOptimizer):
     for k in self._kinds:
       k.rec["step"] = counts[k.mine]
     if self._on_device:
-      self._steps_dev.copy_(torch.from_numpy(counts.copy()))
+      self._steps_dev[:, 0] = torch.from_numpy(counts.copy()).to(self.device)
 
   def state_dict(self):
     """Everything a resumed run needs: counts, options and copies of `buffers`."""
@@ -430,7 +425,7 @@ class AdamW(_EngineOptimizer):
       if g is None:
         r["g"], missing = 0, missing + 1
         if kind.grads is not None:
-          kind.grads[j] = (0, 0, 0, 0)
+          kind.grads[j] = (0, 0, 0, -1)
         continue
       if g.layout != torch.strided:
         raise ValueError("gradients must be dense tensors, got %s" % g.layout)
@@ -448,7 +443,7 @@ class AdamW(_EngineOptimizer):
         copies.append(g)
       r["p"], r["g"], r["g_type"] = p.data_ptr(), g.data_ptr(), _TYPES[g.dtype]
       if kind.grads is not None:
-        kind.grads[j] = (g.data_ptr(), g.numel(), _TYPES[g.dtype], 0)
+        kind.grads[j] = (g.data_ptr(), g.numel(), _TYPES[g.dtype], r["index"])
     return missing
 
   @torch.no_grad()
@@ -489,14 +484,11 @@ class AdamW(_EngineOptimizer):
     stream = torch.cuda.current_stream(index).cuda_stream
     clip = None
     if self._on_device:
-      which = self._which
-      if partial:
-        which = np.concatenate([rec["index"] for _, rec in todo])
       clip = self._clip.data_ptr()
       norm = self.max_grad_norm
-      _lib.check(L.oivae_grad_norm(self._norm_rec.ctypes.data, 0 if norm is None else len(self._norm_rec), grad_scale,
-                                   0.0 if norm is None else float(norm), clip, self._steps_dev.data_ptr(), which.ctypes.data,
-                                   len(which), self._ws.data_ptr(), self._ws.numel(), stream), "oivae_grad_norm")
+      _lib.check(L.oivae_grad_norm(self._norm_rec.ctypes.data, len(self._norm_rec), norm is not None, grad_scale,
+                                   0.0 if norm is None else float(norm), clip, self._steps_dev.data_ptr(), b1, b2,
+                                   self._ws.data_ptr(), self._ws.numel(), stream), "oivae_grad_norm")
     for k, rec in todo:
       if not len(rec):
         continue

@@ -29,13 +29,13 @@ def test_record_sizes_are_those_of_the_header(tmp_path):
   lib, _ = _lib()
   root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
   src = tmp_path / "sizes.c"
-  src.write_text('#include "oivae_hip.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(void) { printf("%zu %zu %zu %zu %zu %zu %d",'
+  src.write_text('#include "oivae_hip.h"\n#include <stdio.h>\n#include <stddef.h>\nint main(void) { printf("%zu %zu %zu %zu %zu %zu %zu %d",'
                  'sizeof(oivae_grad_t), sizeof(oivae_adamw_tensor_t), sizeof(oivae_adamw_group_t), sizeof(oivae_adamw_state_t),'
-                 'sizeof(oivae_clip_t), offsetof(oivae_adamw_tensor_t, step), OIVAE_ADAMW_BLOCK); return 0; }\n')
+                 'sizeof(oivae_clip_t), sizeof(oivae_step_t), offsetof(oivae_adamw_tensor_t, step), OIVAE_ADAMW_BLOCK); return 0; }\n')
   exe = tmp_path / "sizes"
   subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
   got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
-  assert got == [optim._GRAD.itemsize, optim._TENSOR.itemsize, optim._GROUP.itemsize, ctypes.sizeof(lib.AdamwState), 16,
+  assert got == [optim._GRAD.itemsize, optim._TENSOR.itemsize, optim._GROUP.itemsize, ctypes.sizeof(lib.AdamwState), 32, 16,
                  optim._TENSOR.fields["step"][1], lib.ADAMW_BLOCK]
 
 
@@ -74,15 +74,16 @@ def test_entry_points_refuse_bad_calls():
   g = np.zeros(2, optim._GRAD)
   g["g"], g["n"] = 4096, 10
   need = L.oivae_grad_norm_workspace_bytes(2)
-  norm = lambda clip=1 << 20, steps=None, which=None, n=0, ws=2 << 20, nb=need, count=2, rec=g: L.oivae_grad_norm(
-    rec.ctypes.data, count, 1.0, 1.0, clip, steps, which, n, ws, nb, None)
-  idx = np.array([0, -1], np.int32)
-  assert norm(clip=None) == 1 and norm(count=-1) == 1 and norm(n=2) == 1 and norm(n=-1) == 1
-  assert norm(steps=1 << 20, which=idx.ctypes.data, n=2) == 1
-  assert norm(ws=None) == 4 and norm(nb=need - 1) == 4 and norm(ws=(2 << 20) + 4) == 4
-  assert L.oivae_grad_clip(g.ctypes.data, 2, None, None) == 1
-  g["type"][1] = 7
-  assert norm() == 1 and L.oivae_grad_clip(g.ctypes.data, 2, 1 << 20, None) == 1
+  norm = lambda clip=1 << 20, steps=None, b1=0.9, ws=2 << 20, nb=need, count=2, rec=g.ctypes.data: L.oivae_grad_norm(
+    rec, count, 1, 1.0, 1.0, clip, steps, b1, 0.999, ws, nb, None)
+  scale = lambda out=1 << 20, ws=2 << 20, nb=need, count=2, rec=g.ctypes.data: L.oivae_clip_grad_norm(rec, count, 1.0, out, ws, nb, None)
+  assert norm(clip=None) == 1 and norm(steps=1 << 20, b1=1.0) == 1 and scale(out=None) == 1
+  for call in (norm, scale):
+    assert call(count=-1) == 1 and call(rec=None) == 1 and call(ws=None) == 4 and call(nb=need - 1) == 4 and call(ws=(2 << 20) + 4) == 4
+  for field, bad in (("type", 7), ("type", -1), ("index", -2), ("index", 1 << 29), ("n", -1), ("g", 0), ("g", 4098)):
+    keep, g[field][1] = g[field][1], bad
+    assert norm() == 1 and scale() == 1, (field, bad)
+    g[field][1] = keep
   assert L.oivae_grad_norm_workspace_bytes(0) >= 8 and L.oivae_grad_norm_workspace_bytes(10000) > need
 
 
