@@ -31,6 +31,11 @@ bool plain(const at::Tensor& t, int device) {
          (t.is_contiguous() || t.is_non_overlapping_and_dense());
 }
 
+// what autograd is told where a kernel writes a tensor behind its back: a graph that saved it says so instead of going on
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 struct Buffer {
   Py_buffer b;
   bool held = false;
@@ -81,6 +86,7 @@ PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (!plain(p, (int)device) || !plain(g, (int)device) || p.numel() != r[i].n || type_of(p) != r[i].p_type || !g.sizes().equals(p.sizes()))
         break;
       if (!(p.is_contiguous() && g.is_contiguous()) && !g.strides().equals(p.strides())) break;
+      written(p);
       r[i].p = p.data_ptr();
       r[i].g = g.data_ptr();
       r[i].g_type = type_of(g);
@@ -94,14 +100,15 @@ PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return Py_BuildValue("(nl)", unusual, missing);
 }
 
-// gradients(list, records of oivae_grad_t) -> (count, device) of the gradients that are there, or None when one is unusual,
+// gradients(list, records of oivae_grad_t, whether they will be written) -> (count, device) of the gradients that are there, or None when one is unusual,
 // appears twice or is on another device; (0, -1) without any.
 PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 2 || !PyList_Check(args[0])) {
-    PyErr_SetString(PyExc_TypeError, "gradients(list, records)");
+  if (nargs != 3 || !PyList_Check(args[0])) {
+    PyErr_SetString(PyExc_TypeError, "gradients(list, records, written)");
     return nullptr;
   }
   const Py_ssize_t n = PyList_GET_SIZE(args[0]);
+  const bool write = args[2] == Py_True;
   Buffer buf;
   if (!buf.take(args[1], sizeof(oivae_grad_t), n)) return nullptr;
   oivae_grad_t* r = static_cast<oivae_grad_t*>(buf.b.buf);
@@ -122,6 +129,10 @@ PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     std::sort(seen.begin(), seen.end());
     if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
+    for (Py_ssize_t i = 0; write && i < n; ++i) {
+      const at::Tensor& g = THPVariable_Unpack(PyList_GET_ITEM(args[0], i)).grad();
+      if (g.defined()) written(g);
+    }
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;

@@ -151,12 +151,18 @@ def _lists():
 _lists_module = None
 
 
-def _grads_of(parameters):
+def _written(t):
+  """Tells autograd that a kernel writes t."""
+  if not t.is_inference():
+    torch.autograd.graph.increment_version(t)
+
+
+def _grads_of(parameters, write):
   """(records, device index, gradients, their dense copies where they are not one piece of memory) of the gradients that
   are there; None without any."""
   ps = [parameters] if torch.is_tensor(parameters) else list(parameters)
   rec = np.zeros(len(ps), _GRAD)
-  got = _lists().gradients(ps, rec)
+  got = _lists().gradients(ps, rec, write)
   if got is not None:
     count, device = got
     return (rec[:count], device, (), ()) if count else None
@@ -175,6 +181,9 @@ def _grads_of(parameters):
 
 
 def _clip(rec, device, max_norm):
+  if torch.cuda.current_device() != device:
+    with torch.cuda.device(device):
+      return _clip(rec, device, max_norm)
   L = _lib.init_device(device)
   nbytes = L.oivae_grad_norm_workspace_bytes(len(rec))
   # norm and workspace of this call alone: calls on other streams and in captured graphs have their own
@@ -188,11 +197,10 @@ def grad_norm(parameters):
   """2-norm of the gradients of `parameters` (a tensor or an iterable of tensors; those without a gradient are left out)
   taken as one vector: a 0-dim float32 tensor on their device, with no synchronisation.  Squares and sums are formed in
   fp64, in an order that depends on the sizes alone."""
-  got = _grads_of(parameters)
+  got = _grads_of(parameters, False)
   if got is None:
     return torch.zeros(())
-  with torch.cuda.device(got[1]):
-    return _clip(got[0], got[1], 0.0)
+  return _clip(got[0], got[1], 0.0)
 
 
 def clip_grad_norm_(parameters, max_norm):
@@ -201,16 +209,18 @@ def clip_grad_norm_(parameters, max_norm):
   max_norm = float(max_norm)
   if not max_norm > 0:
     raise ValueError("max_norm must be positive, got %r" % max_norm)
-  got = _grads_of(parameters)
+  got = _grads_of(parameters, True)
   if got is None:
     return torch.zeros(())
   rec, device, grads, packed = got
-  with torch.cuda.device(device):
-    norm = _clip(rec, device, max_norm)
+  norm = _clip(rec, device, max_norm)
+  if grads:
     with torch.no_grad():
       for g, c in zip(grads, packed):
         if c is not g:
           g.copy_(c)
+        else:
+          _written(g)
   return norm
 
 
@@ -316,10 +326,13 @@ class AdamW(_EngineOptimizer):
       if mine:
         self._kinds.append(_Kind(self, bits, mine, groups))
     buffers = {k.bits: k.held for k in self._kinds}
+    self._groups = np.zeros(len(self.param_groups), _GROUP)
+    self._groups_at = self._groups.ctypes.data
     self._clip = torch.zeros(8, dtype=torch.int32, device=device) if self._on_device else None
     if self._on_device:
       self._ws = torch.empty(self._lib.oivae_grad_norm_workspace_bytes(len(leaves)), dtype=torch.uint8, device=device)
       self._norm_rec = np.zeros(len(leaves), _GRAD)   # the gradients of all kinds, one behind the other
+      self._norm_at = self._norm_rec.ctypes.data
       at = 0
       for k in self._kinds:
         k.grads = self._norm_rec[at:at + len(k.mine)]
@@ -391,7 +404,7 @@ class AdamW(_EngineOptimizer):
   def state_dict(self):
     """Everything a resumed run needs: counts, options and copies of `buffers`."""
     return {"steps": self.steps(), "seed": self.seed,
-            "groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups],
+            "groups": [{k: v.clone() if torch.is_tensor(v) else v for k, v in g.items() if k != "params"} for g in self.param_groups],
             "buffers": {bits: {k: t.clone() for k, t in held.items()} for bits, held in self.buffers.items()}}
 
   @torch.no_grad()
@@ -411,9 +424,16 @@ class AdamW(_EngineOptimizer):
     self.set_steps(state["steps"])
     self.seed = state["seed"]
     for g, src in zip(self.param_groups, state["groups"]):
-      g.update(src)
+      if any(src[k] != g[k] for k in ("state_bits",)):
+        raise ValueError("the state holds other state_bits")
+      for k, v in src.items():
+        if torch.is_tensor(g[k]):
+          g[k].copy_(torch.as_tensor(v))     # an lr on the device stays where a captured graph reads it
+        else:
+          g[k] = v.item() if torch.is_tensor(v) else v
 
   # ---- the step ---------------------------------------------------------------
+  @torch.no_grad()
   def _read(self, kind, copies):
     """Addresses of a kind's parameters and gradients into its records, the way round (csrc/tensor_lists.cpp takes lists
     that are all as their records say): copies gradients into their parameter's order, says what cannot be stepped.
@@ -441,12 +461,12 @@ class AdamW(_EngineOptimizer):
       if g.is_neg() or (g.stride() != p.stride() and not (p.is_contiguous() and g.is_contiguous())):
         g = torch.empty_like(p, dtype=g.dtype).copy_(g)
         copies.append(g)
+      _written(p)
       r["p"], r["g"], r["g_type"] = p.data_ptr(), g.data_ptr(), _TYPES[g.dtype]
       if kind.grads is not None:
         kind.grads[j] = (g.data_ptr(), g.numel(), _TYPES[g.dtype], r["index"])
     return missing
 
-  @torch.no_grad()
   def step(self, grad_scale=1.0):
     """One step from the parameters' gradients, times grad_scale (1 / loss scale).  Parameters without a gradient stay as
     they are and keep their count, as in torch.optim."""
@@ -459,14 +479,22 @@ class AdamW(_EngineOptimizer):
         self._step(float(grad_scale))
 
   def _step(self, grad_scale):
-    (b1, b2), eps = self._uniform("betas"), self._uniform("eps")
-    L, index = self._lib, self.device.index
+    first, L, index = self.param_groups[0], self._lib, self.device.index
+    (b1, b2), eps = first["betas"], first["eps"]
+    groups = self._groups
+    for q, g in enumerate(self.param_groups):
+      if g is not first and (g["eps"] != eps or tuple(g["betas"]) != (b1, b2)):
+        raise ValueError("AdamW applies one 'betas' and one 'eps' to every param group")
+      lr = g["lr"]
+      groups[q] = self._lr_on_device(lr, g) if torch.is_tensor(lr) else (lr, g["weight_decay"], 0)
+    if self.max_grad_norm is not None and not self._on_device:
+      raise RuntimeError("max_grad_norm has to be given to the constructor (it may be changed or set to None later)")
     if not self._on_device and torch.cuda.is_current_stream_capturing():
       raise RuntimeError("a captured step would repeat its step count at every replay: use AdamW(capturable=True)")
-    groups = np.array([self._group_options(g) for g in self.param_groups], _GROUP)
     todo, partial, copies = [], False, []
     for k in self._kinds:
       if self._engine is not None:
+        self._uniform("lr"), self._uniform("weight_decay")   # one for the flat buffer, whatever a schedule does
         k.rec["p"], k.rec["g"] = self._leaves[0].data_ptr(), self._engine.flat_grads.data_ptr()
         if k.grads is not None:
           k.grads[0] = (k.rec["g"][0], k.rec["n"][0], _lib.F32, 0)
@@ -486,31 +514,32 @@ class AdamW(_EngineOptimizer):
     if self._on_device:
       clip = self._clip.data_ptr()
       norm = self.max_grad_norm
-      _lib.check(L.oivae_grad_norm(self._norm_rec.ctypes.data, len(self._norm_rec), norm is not None, grad_scale,
+      _lib.check(L.oivae_grad_norm(self._norm_at, len(self._norm_rec), norm is not None, grad_scale,
                                    0.0 if norm is None else float(norm), clip, self._steps_dev.data_ptr(), b1, b2,
                                    self._ws.data_ptr(), self._ws.numel(), stream), "oivae_grad_norm")
     for k, rec in todo:
       if not len(rec):
         continue
+      counts = k.rec["step"]
       if not self._on_device:
-        if rec is k.rec:
+        counts += 1
+        if rec is not k.rec:
+          counts[k.rec["g"] == 0] -= 1
           rec["step"] += 1
-        else:
-          k.rec["step"][k.rec["g"] != 0] += 1
-          rec["step"] += 1
-      args = (rec.ctypes.data, len(rec), groups.ctypes.data, len(groups), k.state_ref, b1, b2, eps, grad_scale)
+      args = (k.rec_at if rec is k.rec else rec.ctypes.data, len(rec), self._groups_at, len(groups), k.state_ref, b1, b2, eps, grad_scale)
       if k.bits == 32:
-        _lib.check(L.oivae_adamw_f32(*args, clip, stream), "oivae_adamw_f32")
+        rc = L.oivae_adamw_f32(*args, clip, stream)
       else:
-        _lib.check(L.oivae_adamw_f8(*args, self.seed, clip, stream), "oivae_adamw_f8")
+        rc = L.oivae_adamw_f8(*args, self.seed, clip, stream)
+      if rc:
+        if not self._on_device:
+          counts[k.rec["g"] != 0] -= 1
+        _lib.check(rc, "oivae_adamw_f%d" % k.bits)
 
-  def _group_options(self, g):
-    lr = g["lr"]
-    if not torch.is_tensor(lr):
-      return lr, g["weight_decay"], 0
+  def _lr_on_device(self, lr, group):
     if lr.numel() != 1 or lr.dtype != torch.float32 or lr.device != self.device:
       raise ValueError("an lr tensor must be one float32 on %s" % self.device)
-    return 0.0, g["weight_decay"], lr.data_ptr()
+    return 0.0, group["weight_decay"], lr.data_ptr()
 
 
 class _Kind(object):
@@ -526,6 +555,7 @@ class _Kind(object):
     rec["p_type"] = [_TYPES[p.dtype] for p in self.leaves]
     rec["group"] = [groups[i] for i in mine]
     rec["index"] = mine
+    self.rec_at = rec.ctypes.data
     total, half = max(int(whole.sum()), _lib.ADAMW_BLOCK), int(whole[rec["p_type"] != _lib.F32].sum())
     self.held = held = {}
     if bits == 32:

@@ -27,12 +27,13 @@ def adamw64(w, g, m, v, t, lr, b1, b2, eps, wd):
   return w2, m2, v2, tol_w, tol_m, tol_v
 
 
-def random_bits(seed, step, tensor, n):
+def random_bits(seed, step, tensor, n, first=0):
   k = (seed * C1 + step * C3 + tensor * C4) & M32
   k = ((k ^ (k >> 16)) * C2) & M32
   k = ((k ^ (k >> 15)) * C3) & M32
   k ^= k >> 16
-  x = (np.arange(n, dtype=np.uint64) * C1 + k) & M32
+  i = np.arange(first, first + n, dtype=np.uint64)
+  x = ((i & M32) * C1 + (i >> np.uint64(32)) * C4 + k) & M32
   x = ((x ^ (x >> 14)) * C2) & M32
   return (x ^ (x >> 14)).astype(np.int64)
 

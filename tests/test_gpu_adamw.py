@@ -286,11 +286,12 @@ def test_what_is_not_finite_stays_visible():
 
 
 # ---- norm and clipping -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("offset", [0, 1, 3])
 @pytest.mark.parametrize("typ", list(TYPES))
 @pytest.mark.parametrize("sizes", list(SIZES))
-def test_norm_and_clipping(sizes, typ):
+def test_norm_and_clipping(sizes, typ, offset):
   from oi_vae_amd import optim
-  ps = _params(SIZES[sizes], TYPES[typ], seed=11)
+  ps = _params(SIZES[sizes], TYPES[typ], seed=11, offset=offset)
   g = [_np(p.grad) for p in ps]
   norm = np.sqrt(sum((x * x).sum() for x in g))
   got = optim.grad_norm(ps)
@@ -347,17 +348,19 @@ def test_norm_of_extreme_and_odd_gradients():
 
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("typ", list(TYPES))
-def test_clipped_step(typ, bits):
-  ps = _params(SIZES["blocks"], TYPES[typ], seed=4)
+@pytest.mark.parametrize("sizes", ["blocks", "many", "long", "several thousand blocks"])
+def test_clipped_step(sizes, typ, bits):
+  sizes = SIZES.get(sizes, [9000000, 5])     # one launch, two, more partial sums than one launch concludes, more than its blocks
+  ps = _params(sizes, TYPES[typ], seed=4)
   opt = _opt(ps, 9, lr=1e-3, weight_decay=0.1, state_bits=bits, max_grad_norm=0.05)
   before = _state(opt)
   grads = [_np(p.grad) for p in ps]
   norm = 0.5 * np.sqrt(sum((x * x).sum() for x in grads))
   opt.step(grad_scale=0.5)
   assert abs(opt.grad_norm.item() - norm) <= 2 * U * norm and norm > 0.05
-  _check(opt, before, _state(opt), grads, 9, [1e-3] * 6, [0.1] * 6, scale=0.5 * 0.05 / (norm + 1e-6), codes=False)
+  _check(opt, before, _state(opt), grads, 9, [1e-3] * len(ps), [0.1] * len(ps), scale=0.5 * 0.05 / (norm + 1e-6), codes=False)
   assert all(np.array_equal(_np(p.grad), g) for p, g in zip(ps, grads))
-  assert opt.steps() == [9] * 6 and opt.skipped.item() == 0
+  assert opt.steps() == [9] * len(ps) and opt.skipped.item() == 0
 
 
 @pytest.mark.parametrize("bits", [32, 8])
@@ -375,6 +378,97 @@ def test_a_step_whose_norm_is_not_finite_is_left_out(bits):
     ps[1].grad[17] = 0.0
     opt.step()
     assert opt.skipped.item() == 1 and opt.steps() == [4, 4] and not torch.equal(ps[0], was[0])
+
+
+def test_tiny_and_zero_eps():
+  """eps below what the hardware's root can hold, and none: gradients down to float32's subnormal squares."""
+  from oi_vae_amd import optim
+  g = torch.tensor(10.0 ** np.linspace(-21, 3, 1000), dtype=torch.float32, device="cuda")
+  for eps in (0.0, 1e-18, 1e-12):
+    for bits in (32, 8):
+      p = torch.zeros(1000, device="cuda").requires_grad_()
+      p.grad = g.clone()
+      optim.AdamW([p], lr=1e-3, eps=eps, weight_decay=0.0, state_bits=bits).step()
+      x = _np(g)
+      v = (np.float32(1 - B2) * g.cpu().numpy() ** 2).astype(np.float64)      # as far as float32 holds it
+      live = v > 2.0 ** -126
+      want = -1e-3 * x / (np.sqrt(x * x) + eps)
+      assert np.all(np.abs(_np(p) - want)[live] <= 64 * U * np.abs(want)[live]), (eps, bits)
+  # nothing at all: 0 / 0 without eps, as the formula says; zero with it
+  for eps, same in ((0.0, False), (1e-8, True)):
+    for bits in (32, 8):
+      p = torch.ones(5, device="cuda").requires_grad_()
+      p.grad = torch.zeros(5, device="cuda")
+      optim.AdamW([p], lr=1e-3, eps=eps, weight_decay=0.0, state_bits=bits).step()
+      assert bool((p == 1).all()) == same and bool(torch.isnan(p).all()) != same
+
+
+@pytest.mark.parametrize("b1,b2", [(0.0, 0.999), (0.9, 0.0), (0.0, 0.0), (0.5, 0.9999999)])
+def test_other_betas(b1, b2):
+  from oi_vae_amd import optim
+  for kw in (dict(), dict(capturable=True)):
+    for bits in (32, 8):
+      p = _params([300], torch.float32, seed=3)[0]
+      w, g = _np(p), _np(p.grad)
+      optim.AdamW([p], lr=1e-2, betas=(b1, b2), eps=EPS, weight_decay=0.1, state_bits=bits, **kw).step()
+      want = w * (1 - 1e-3) - 1e-2 * g / (np.abs(g) + EPS)        # the first step, whatever the betas
+      assert np.all(np.abs(_np(p) - want) <= 4 * U * np.abs(w) + 64 * U * 1e-2 + 2 * U * np.abs(want)), (kw, bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_2_to_the_32_elements(bits):
+  """Offsets past 32 bits in the tensor, its moments and its random bits (bfloat16; about 60 GB with moments in 32 bits)."""
+  from oi_vae_amd import optim
+  n = (1 << 32) + 5003
+  if torch.cuda.mem_get_info()[0] < 80 << 30:
+    pytest.skip("needs 80 GB")
+  p = torch.zeros(n, dtype=torch.bfloat16, device="cuda").requires_grad_()
+  p.grad = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+  opt = optim.AdamW([p], lr=1e-2, weight_decay=0.0, state_bits=bits, max_grad_norm=1e9)
+  spots = [(0, 4096), ((1 << 31) - 2048, 4096), ((1 << 32) - 2048, 4096), (n - 1000, 1000)]
+  g = torch.Generator(device="cuda").manual_seed(0)
+  for a, k in spots:
+    p.grad[a:a + k] = torch.randn(k, generator=g, device="cuda").bfloat16()
+  norm = np.sqrt(sum((_np(p.grad[a:a + k]) ** 2).sum() for a, k in spots))
+  opt.step()
+  assert abs(opt.grad_norm.item() - norm) <= 2 * U * norm
+  held = opt.buffers[bits]
+  for a, k in spots:
+    x = _np(p.grad[a:a + k])
+    want = -1e-2 * x / (np.abs(x) + EPS)
+    assert np.all(np.abs(_np(held["master"][a:a + k]) - want) <= 64 * U * 1e-2)
+    lo = a // 128 * 128
+    if bits == 8:
+      full = np.zeros(a + k - lo)
+      full[a - lo:] = x
+      m32, v32 = moments32(full, 0 * full, 0 * full, B1, B2)
+      noise = random_bits(0, 1, 0, len(full), first=lo)
+      for name, val, digits, r in (("exp_avg", m32, 3, (noise >> 12) / 2.0 ** 20), ("exp_avg_sq", v32, 2, (noise & 0x1FFFFF) / 2.0 ** 21)):
+        c, b = encode(val, digits, r)
+        assert np.array_equal(held[name].view(torch.uint8)[lo:a + k].cpu().numpy(), c), (name, a)
+    else:
+      m = 0.1 * x
+      assert np.all(np.abs(_np(held["exp_avg"][a:a + k]) - m) <= 4 * U * np.abs(m))
+  assert (p[5000:1 << 20] == 0).all()
+  got = optim.clip_grad_norm_(p, norm / 2)
+  assert abs(got.item() - norm) <= 2 * U * norm
+  a, k = spots[-1]
+  assert abs(_np(p.grad[a:a + k])).max() > 0 and abs(optim.grad_norm(p).item() - norm / 2) <= 2.0 ** -8 * norm
+  del p, opt, held
+  torch.cuda.empty_cache()
+
+
+def test_autograd_hears_of_the_step():
+  """A graph that saved a weight refuses to run backward after the step, as behind torch.optim."""
+  from oi_vae_amd import optim
+  for shape in ((4, 4), (4, 8)):
+    w = torch.randn(8, 8, device="cuda")[:, :shape[1]].t().contiguous().t().requires_grad_()
+    x = torch.randn(3, 8, device="cuda", requires_grad=True)
+    loss = ((x @ w) ** 2).sum()
+    loss.backward(retain_graph=True)
+    optim.AdamW([w], lr=0.1).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+      loss.backward()
 
 
 # ---- streams, graphs, resuming ---------------------------------------------------------------------------------------------
