@@ -265,8 +265,8 @@ __device__ __forceinline__ void conclude(const GradLaunch& a, const double* part
     const int t = q.t + 1;
     q.t = t;
     // 1 - b^t = -expm1(t ln b) keeps its digits where b^t is near 1 (t = 1, b2 = 0.999)
-    q.inv_bc1 = (float)(1.0 / -expm1(t * v.ln_b1));
-    q.inv_bc2_sqrt = (float)(1.0 / sqrt(-expm1(t * v.ln_b2)));
+    q.inv_bc1 = 1.f / -expm1f((float)(t * v.ln_b1));
+    q.inv_bc2_sqrt = 1.f / sqrtf(-expm1f((float)(t * v.ln_b2)));
   }
 }
 

@@ -25,7 +25,9 @@ class Experiment(object):
 
   def __init__(self, dim_x, dim_z, group_dims, group_input_dim, gen_type="linear", hidden=0,
                lr=1e-3, Ws_lr=1e-4, lam=1.0, lam_adjustment=1.0, prior_theta_scale=1.0,
-               prior_rows=1, native_optimizers=True, device=None, device_eps=False):
+               prior_rows=1, native_optimizers=True, device=None, device_eps=False,
+               weight_decay=None, state_bits=32, max_grad_norm=None):
+    """weight_decay (a number): the engine's AdamW instead of Adam, with its state_bits and max_grad_norm."""
     assert sum(group_dims) == dim_x
     self.stddev_multiple = 0.1  # bars_data_oivae.py:60; read through the closure below on every step
     self.lam, self.lam_adjustment, self.Ws_lr = lam, lam_adjustment, Ws_lr
@@ -63,7 +65,11 @@ class Experiment(object):
     sgd_groups = [{'params': [self.generative_net.Ws], 'lr': Ws_lr, 'momentum': 0}]
     if native_optimizers:  # the engine's fused Adam and SGD+prox kernels
       from . import optim
-      self.optimizer, self.optimizer_Ws = optim.Adam(adam_groups), optim.SGD(sgd_groups)
+      if weight_decay is None:
+        self.optimizer = optim.Adam(adam_groups)
+      else:
+        self.optimizer = optim.AdamW(adam_groups, weight_decay=weight_decay, state_bits=state_bits, max_grad_norm=max_grad_norm)
+      self.optimizer_Ws = optim.SGD(sgd_groups)
     else:                  # caller-owned torch.optim, exactly as the scripts build them
       self.optimizer, self.optimizer_Ws = torch.optim.Adam(adam_groups), torch.optim.SGD(sgd_groups)
     prior_z = Normal(torch.zeros(prior_rows, dim_z), torch.ones(prior_rows, dim_z))

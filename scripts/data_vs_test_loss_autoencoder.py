@@ -17,6 +17,7 @@ import sys
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from oi_vae_amd import optim  # noqa: E402
 from oi_vae_amd.bars_data import sample_bars_image  # noqa: E402
 from oi_vae_amd.models import FirstLayerSparseDecoder  # noqa: E402
 
@@ -55,6 +56,11 @@ def main(argv=None):
   ap.add_argument("--lams", type=float, nargs="+", default=[0.0, 0.1])     # :24
   ap.add_argument("--test-samples", type=int, default=2048)
   ap.add_argument("--linear-decoder", action="store_true")
+  ap.add_argument("--optimizer", choices=("adam", "adamw"), default="adam",
+                  help="torch.optim.Adam as the reference, or oi_vae_amd.optim.AdamW (one kernel for all tensors)")
+  ap.add_argument("--weight-decay", type=float, default=0.0, help="adamw: decoupled weight decay")
+  ap.add_argument("--state-bits", type=int, choices=(8, 32), default=32, help="adamw: bits of the moments")
+  ap.add_argument("--max-grad-norm", type=float, default=None, help="adamw: clip the gradients by their norm")
   ap.add_argument("--out", default="out_autoencoder/data_vs_test_loss.json")
   args = ap.parse_args(argv)
   if not torch.cuda.is_available():
@@ -70,7 +76,11 @@ def main(argv=None):
     for lam in args.lams:
       encoder = torch.nn.Linear(image_size * image_size, dim_z, bias=False).to(dev)
       decoder = (linear_decoder if args.linear_decoder else nonlinear_decoder)(image_size, dim_z).cuda()
-      opt = torch.optim.Adam([{"params": encoder.parameters(), "lr": lr}, {"params": list(decoder.parameters()), "lr": lr}])
+      groups = [{"params": encoder.parameters(), "lr": lr}, {"params": list(decoder.parameters()), "lr": lr}]
+      if args.optimizer == "adam":
+        opt = torch.optim.Adam(groups)
+      else:
+        opt = optim.AdamW(groups, weight_decay=args.weight_decay, state_bits=args.state_bits, max_grad_norm=args.max_grad_norm)
       curves = torch.zeros(args.epochs, 3, device=dev)   # per epoch: test loss, train loss, lam * penalty (kept on the device)
       collapsed = 0
       for ep in range(args.epochs):

@@ -47,6 +47,9 @@ def main(argv=None):
   ap.add_argument("--log-every", type=int, default=50)
   ap.add_argument("--test-fraction", type=float, default=0.1,
                   help="frames held out for the test log-likelihood the reference leaves stubbed (meg_oi_vae.py:258-260)")
+  ap.add_argument("--weight-decay", type=float, default=None, help="AdamW with this decay instead of Adam")
+  ap.add_argument("--state-bits", type=int, choices=(8, 32), default=32, help="bits of AdamW's moments")
+  ap.add_argument("--max-grad-norm", type=float, default=None, help="clip AdamW's gradients by their norm")
   ap.add_argument("--out", default="out_meg")
   args = ap.parse_args(argv)
 
@@ -68,7 +71,8 @@ def main(argv=None):
   batch_size, mc_samples = 4096, 1
   exp = Experiment(dim_x=X.shape[1], dim_z=args.dim_z, group_dims=group_output_dims, group_input_dim=1,
                    gen_type="linear", lr=1e-3, Ws_lr=1e-6, lam=1.0, prior_rows=1,
-                   device=torch.device("cuda", local_rank))
+                   device=torch.device("cuda", local_rank), weight_decay=args.weight_decay, state_bits=args.state_bits,
+                   max_grad_norm=args.max_grad_norm)
   n_test = int(X.shape[0] * args.test_fraction)
   Xtest = torch.from_numpy(X[X.shape[0] - n_test:]).to(exp.device) if n_test else None
   Xd = torch.from_numpy(X[:X.shape[0] - n_test]).to(exp.device)

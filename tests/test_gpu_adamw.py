@@ -678,6 +678,36 @@ def test_oivae_trains_with_adamw(bits, clip, B):
       assert abs(opt.grad_norm.item() - norm) <= 2 * U * norm
 
 
+def test_oivae_steps_adamw_behind_the_gradient_reduction(monkeypatch):
+  """The data-parallel order of OIVAE.step: AdamW runs once, after both buckets are reduced (here by a stand-in that doubles
+  the gradients when they are waited for)."""
+  from oi_vae_amd import optim, parallel
+
+  class Sync:
+    def __init__(self, holder, group=None):
+      self.flat = holder.flat_grads
+
+    def decoder_grads_ready(self):
+      pass
+
+    encoder_grads_ready = decoder_grads_ready
+
+    def wait(self):
+      self.flat.mul_(2.0)
+  monkeypatch.setattr(parallel, "is_active", lambda group=None: True)
+  monkeypatch.setattr(parallel, "BucketedGradSync", Sync)
+  monkeypatch.setattr(parallel, "reduce_scalars_", lambda scalars, group=None: scalars)
+  vae, (opt, _) = _vae(lambda groups, ws: [optim.AdamW(groups, lr=1e-3, weight_decay=0.05, max_grad_norm=1.0), optim.SGD(ws, lr=1e-4)])
+  X = torch.rand(16, 24, generator=torch.Generator().manual_seed(1)).cuda()
+  for t in (1, 2):
+    before = _state(opt)
+    vae.step(X, 1e-3, 1)
+    g = _np(vae.engine.flat_grads[:vae.engine.adam_numel])
+    norm = np.sqrt((g * g).sum())
+    _check(opt, before, _state(opt), [g], t, [1e-3], [0.05], scale=min(1.0, 1.0 / (norm + 1e-6)))
+    assert abs(opt.grad_norm.item() - norm) <= 2 * U * norm
+
+
 def test_engine_adamw_is_one_option_set():
   from oi_vae_amd import optim
   with pytest.raises(ValueError, match="weight_decay"):
@@ -727,6 +757,29 @@ def test_steps_queued_behind_a_failed_decoder_change_nothing():
       opt.step()
       torch.cuda.synchronize()
       assert not torch.equal(p, before)
+
+
+def _script(name):
+  import importlib.util
+  import os
+  path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "scripts", name + ".py")
+  spec = importlib.util.spec_from_file_location(name, path)
+  mod = importlib.util.module_from_spec(spec)
+  spec.loader.exec_module(mod)
+  return mod
+
+
+@pytest.mark.parametrize("bits", ["32", "8"])
+def test_drivers_run_with_adamw(tmp_path, bits):
+  common = ["--weight-decay", "0.01", "--state-bits", bits, "--max-grad-norm", "10"]
+  res = _script("data_vs_test_loss_autoencoder").main(["--epochs", "30", "--train-sizes", "8", "--lams", "0.1", "--test-samples", "64",
+                                                       "--optimizer", "adamw", "--out", str(tmp_path / "a.json")] + common)
+  assert len(res) == 1 and np.all(np.isfinite(res[0]["test_loss"])) and len(set(res[0]["train_loss"])) == 30
+  exp = _script("meg_oi_vae").main(["--labels", "12", "--frames", "10000", "--max-iterations", "8", "--log-every", "4",
+                                    "--out", str(tmp_path / "meg")] + common)
+  opt = exp.optimizer
+  assert opt.steps() == [8] and opt.skipped.item() == 0 and np.isfinite(opt.grad_norm.item())
+  assert list(opt.buffers) == [int(bits)] and torch.isfinite(exp.vae.engine.flat_params).all()
 
 
 def test_pointers_are_read_at_every_call():
