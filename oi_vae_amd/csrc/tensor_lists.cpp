@@ -100,8 +100,9 @@ PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return Py_BuildValue("(nl)", unusual, missing);
 }
 
-// gradients(list, records of oivae_grad_t, whether they will be written) -> (count, device) of the gradients that are there, or None when one is unusual,
-// appears twice or is on another device; (0, -1) without any.
+// gradients(list, records of oivae_grad_t, whether they will be written) -> (count, device, address of the
+// records) of the gradients that are there, or None when one is unusual,
+// appears twice or is on another device; (0, -1, address) without any.
 PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 3 || !PyList_Check(args[0])) {
     PyErr_SetString(PyExc_TypeError, "gradients(list, records, written)");
@@ -137,7 +138,7 @@ PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
     return nullptr;
   }
-  return Py_BuildValue("(li)", count, device);
+  return Py_BuildValue("(liK)", count, device, (unsigned long long)reinterpret_cast<uintptr_t>(r));
 }
 
 PyMethodDef methods[] = {

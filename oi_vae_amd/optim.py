@@ -158,14 +158,14 @@ def _written(t):
 
 
 def _grads_of(parameters, write):
-  """(records, device index, gradients, their dense copies where they are not one piece of memory) of the gradients that
-  are there; None without any."""
+  """(records, their number and address, device index, gradients, their dense copies where they are not one piece of memory)
+  of the gradients that are there; None without any."""
   ps = [parameters] if torch.is_tensor(parameters) else list(parameters)
   rec = np.zeros(len(ps), _GRAD)
   got = _lists().gradients(ps, rec, write)
   if got is not None:
-    count, device = got
-    return (rec[:count], device, (), ()) if count else None
+    count, device, address = got
+    return (rec, count, address, device, (), ()) if count else None
   grads = [p.grad for p in ps if p.grad is not None]
   device = _check_types(grads, "gradients")
   if len({g.data_ptr() for g in grads if g.numel()}) != sum(1 for g in grads if g.numel()):
@@ -177,20 +177,21 @@ def _grads_of(parameters, write):
   rec["n"] = [g.numel() for g in packed]
   rec["type"] = [_TYPES[g.dtype] for g in packed]
   rec["index"] = -1
-  return rec, device.index, grads, packed
+  return (rec, len(rec), rec.ctypes.data, device.index, grads, packed) if grads else None
 
 
-def _clip(rec, device, max_norm):
+def _clip(got, max_norm):
+  _, count, address, device = got[:4]
   if torch.cuda.current_device() != device:
     with torch.cuda.device(device):
-      return _clip(rec, device, max_norm)
+      return _clip(got, max_norm)
   L = _lib.init_device(device)
-  nbytes = L.oivae_grad_norm_workspace_bytes(len(rec))
+  nbytes = L.oivae_grad_norm_workspace_bytes(count)
   # norm and workspace of this call alone: calls on other streams and in captured graphs have their own
-  ws = torch.empty(nbytes // 4 + 4, dtype=torch.float32, device=torch.device("cuda", device))
-  _lib.check(L.oivae_clip_grad_norm(rec.ctypes.data, len(rec), max_norm, ws.data_ptr(), ws.data_ptr() + 16, nbytes,
+  norm, ws = torch.empty((), device="cuda"), torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+  _lib.check(L.oivae_clip_grad_norm(address, count, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes,
                                     torch.cuda.current_stream(device).cuda_stream), "oivae_clip_grad_norm")
-  return ws[0]
+  return norm
 
 
 def grad_norm(parameters):
@@ -200,7 +201,7 @@ def grad_norm(parameters):
   got = _grads_of(parameters, False)
   if got is None:
     return torch.zeros(())
-  return _clip(got[0], got[1], 0.0)
+  return _clip(got, 0.0)
 
 
 def clip_grad_norm_(parameters, max_norm):
@@ -212,11 +213,10 @@ def clip_grad_norm_(parameters, max_norm):
   got = _grads_of(parameters, True)
   if got is None:
     return torch.zeros(())
-  rec, device, grads, packed = got
-  norm = _clip(rec, device, max_norm)
-  if grads:
+  norm = _clip(got, max_norm)
+  if got[4]:
     with torch.no_grad():
-      for g, c in zip(grads, packed):
+      for g, c in zip(*got[4:]):
         if c is not g:
           g.copy_(c)
         else:
