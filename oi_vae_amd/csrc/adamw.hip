@@ -422,7 +422,7 @@ __device__ __forceinline__ Tile find_tile(const AdamwLaunch& a) {
 
 // One vector of four elements per thread and stream: the loads of a wave are 1 KiB pieces, and a small workgroup keeps its
 // four streams short, so that many are in flight.  1024 elements a workgroup against 2048 / 4096 on 268M bf16 parameters:
-// 1279 against 1364 / 1332 us; with weights and moments through the caches 1420 us.
+// 1280 (5.9 TB/s) against 1364 / 1332 us; with weights and moments through the caches 1420 us.
 __global__ __launch_bounds__(kThreads) void adamw32_kernel(AdamwLaunch a) {
   const Tile r = find_tile(a);
   const int64_t i = r.base + threadIdx.x * 4;
@@ -489,9 +489,9 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
 
 // 32 lanes hold one block, four elements each (one vector per thread and stream, as above).  With 16 lanes and 8 elements
 // a lane the vectors of a wave are 32 bytes apart: 861 us on 268M bf16 parameters against 719.
-//   kFast: hardware root and reciprocal (one unit in the last place each) instead of the correctly rounded ones, 45 of 120
-// instructions an element: 719 against 779 us.  The hardware root takes subnormals for zero, an error of 1.1e-19 in the
-// root and of 3.5e-18 in the denominator (t = 1, b2 = 0.999), below its last place while eps >= 1e-10.
+//   kFast: hardware root and reciprocal (one unit in the last place each) instead of the correctly rounded ones, about a
+// third of the instructions: 719 against 779 us (706 now, 6.1 TB/s).  The hardware root takes subnormals for zero: up to
+// 1.1e-19, times 1 / sqrt(1 - b2) at most, in a denominator of at least eps.
 template <bool kFast>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(AdamwLaunch a) {
   const Tile r = find_tile(a);
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(AdamwLaunch a) {
                           : mj[j] / fmaf(sqrtf(vj[j]), r.inv_bc2_sqrt, a.eps);
     wi[j] = fmaf(-r.step_size, q, wi[j] * r.decay);
     mmax = max(mmax, __float_as_uint(mj[j]) & 0x7FFFFFFFu);
-    vmax = max(vmax, __float_as_uint(vj[j]));
+    vmax = max(vmax, __float_as_uint(vj[j]) & 0x7FFFFFFFu);   // (a NaN may carry a sign)
   }
   const uint32_t me = max32(mmax) >> 23, ve = max32(vmax) >> 23;
   const uint32_t mb = me == 255u ? 255u : max(me, 8u) - 7u, vb = ve == 255u ? 255u : max(ve, 15u) - 14u;
@@ -648,13 +648,14 @@ static int run_adamw(const char* who, bool eight, const oivae_adamw_tensor_t* t,
   a.gscale = grad_scale;
   a.seed = seed;
   a.count = 0;
+  const bool fast = eps * sqrt(1.0 - beta2) >= 3e-12;   // what the hardware root loses is under 2^-24 of the denominator
   struct { int32_t group, step; } names[kOptions];
   int32_t n_names = 0;
   uint32_t chunks = 0;
   auto launch = [&]() -> int {
     if (a.count == 0) return OIVAE_OK;
     if (!eight) hipLaunchKernelGGL(adamw32_kernel, dim3(chunks), dim3(kThreads), 0, hs, a);
-    else if (eps >= 1e-10) hipLaunchKernelGGL(adamw8_kernel<true>, dim3(chunks), dim3(kThreads), 0, hs, a);
+    else if (fast) hipLaunchKernelGGL(adamw8_kernel<true>, dim3(chunks), dim3(kThreads), 0, hs, a);
     else hipLaunchKernelGGL(adamw8_kernel<false>, dim3(chunks), dim3(kThreads), 0, hs, a);
     OIVAE_LAUNCH_CHECK();
     a.count = 0;

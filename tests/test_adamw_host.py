@@ -114,3 +114,24 @@ def test_dense_means_one_piece_of_memory():
   x = torch.zeros(4, 6, 5)
   assert all(optim._dense(t) for t in (x, x.permute(2, 0, 1), x[1:3], x.new_zeros(0, 3), x.new_zeros(()), x.new_zeros(1, 7)[:, None]))
   assert not any(optim._dense(t) for t in (x[:, ::2], x[..., :4], x.new_zeros(1).expand(3), x[:, 1:3]))
+
+
+def test_native_reader_leaves_the_unusual_to_python():
+  """csrc/tensor_lists.cpp serves device memory only: a CPU tensor, a list that is none and short records are not read."""
+  from oi_vae_amd import _tensor_lists, optim
+  p, q = torch.zeros(3, requires_grad=True), torch.zeros(3, requires_grad=True)
+  rec, grads = np.zeros(2, optim._TENSOR), np.zeros(2, optim._GRAD)
+  rec["n"] = 3
+  assert _tensor_lists.parameters([p, q], rec, 0, grads) == (-1, 2) and (rec["g"] == 0).all() and (grads["index"] == -1).all()
+  q.grad = torch.ones(3)
+  assert _tensor_lists.parameters([p, q], rec, 0, None) == (1, 1)
+  assert _tensor_lists.parameters([3, q], rec, 0, None)[0] == 0
+  assert _tensor_lists.gradients([p], grads, False)[:2] == (0, -1) and _tensor_lists.gradients([p, q], grads, False) is None
+  assert q.grad._version == 0
+  for bad in (lambda: _tensor_lists.parameters((p,), rec, 0, None), lambda: _tensor_lists.parameters([p], rec, 0), lambda: _tensor_lists.gradients([p])):
+    with pytest.raises(TypeError):
+      bad()
+  with pytest.raises(ValueError, match="fewer records"):
+    _tensor_lists.parameters([p, q, p], rec, 0, None)
+  with pytest.raises(BufferError):
+    _tensor_lists.gradients([p, q], bytes(48), False)
