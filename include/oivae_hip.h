@@ -302,7 +302,7 @@ typedef struct {
   const void* g;     /* gradient (device) */
   int64_t n;
   int64_t at;        /* first element in the moment (and master) buffers: a multiple of OIVAE_ADAMW_BLOCK; the tensor owns
-                        [at, at + n rounded up to whole blocks), which start at zero */
+                        [at, at + n rounded up to whole blocks), which start at zero; places ascend along the list */
   int32_t p_type, g_type;
   int32_t group;     /* index into the groups */
   int32_t index;     /* of its step counter; distinguishes its random bits (oivae_adamw_f8) */
@@ -328,7 +328,8 @@ typedef struct {
 } oivae_adamw_state_t;
 
 /* Norm (with_norm = 0: not computed, zero), coefficient and verdict into `clip`; then, where `steps` is given and the step is
- * not to be left out, the counters of the tensors advance (distinct indices), with the corrections for beta1 and beta2.
+ * not to be left out, the counters of the tensors advance (distinct indices; those below 65536 are checked), with the
+ * corrections for beta1 and beta2.
  * workspace: oivae_grad_norm_workspace_bytes(count) bytes on the device, 8-byte aligned. */
 int64_t oivae_grad_norm_workspace_bytes(int32_t count);
 int oivae_grad_norm(const oivae_grad_t* grads, int32_t count, int32_t with_norm, float grad_scale, float max_norm,

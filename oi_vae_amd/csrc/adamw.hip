@@ -24,7 +24,8 @@ constexpr int kOptions = 8;       // sets of (lr, decay, step) in one launch
 constexpr int kChunk = 1024;      // elements of an AdamW workgroup: one vector of four a thread
 constexpr int kGradSlots = 160;   // tensors of one norm / scaling launch
 constexpr int kNormBlocks = 1024; // cap on the blocks of one norm launch (= its partial sums)
-constexpr int kFewBlocks = 256;   // up to so many, the norm is concluded without a launch of its own
+constexpr int kFewBlocks = 256;   // up to so many, the norm launch concludes the norm itself (grad_norm_one)
+constexpr int kFewChunks = 2048;  // up to so many, the scaling blocks add the partial sums themselves (grad_clip_kernel)
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));        // parameters and gradients may start anywhere
@@ -288,8 +289,9 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const double* __restrict
   if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-// g *= coef, one chunk a block.  With parts > 0 every block adds the partial sums itself (few of them: cheaper than a launch
-// between), and the first one of the first launch leaves the norm.  HBM-bound: 268M fp32 gradients in 410 us behind the norm
+// g *= coef, one chunk a block.  With parts > 0 every block adds the partial sums itself, and the first one of the first launch
+// leaves the norm: cheaper than a launch between for few chunks (5.8M fp16, 800 chunks: norm and scaling 15.6 against 17.5 us),
+// dearer for many (67M bf16, 8264: 76.7 against 75.9; 268M fp32, 65600: 605 against 589).  HBM-bound: 268M fp32 gradients in 410 us behind the norm
 // (5.2 TB/s), 196 us with it when nothing has to be scaled.  One vector a thread scales them in 382 us, but then four times
 // the waves start only to read that the coefficient is one (237 us with the norm).
 __global__ __launch_bounds__(kThreads) void grad_clip_kernel(GradLaunch a, const double* __restrict__ part, int parts, float max_norm,
@@ -589,9 +591,14 @@ static int for_grad_launches(const oivae_grad_t* t, int32_t count, F&& launch) {
 }
 
 static int check_grads(const char* who, const oivae_grad_t* t, int32_t count, void* workspace, int64_t workspace_bytes) {
+  uint64_t seen[1024] = {0};   // indices below 65536: two threads would advance a counter named twice
   for (int32_t i = 0; i < count; ++i) {
     if (int rc = check_grad(who, i, t[i].g, t[i].n, t[i].type)) return rc;
-    if (t[i].index < -1 || t[i].index >= 1 << 29) return fail(OIVAE_E_ARG, "%s: tensor %d has index %d", who, i, t[i].index);
+    const int32_t k = t[i].index;
+    if (k < -1 || k >= 1 << 29) return fail(OIVAE_E_ARG, "%s: tensor %d has index %d", who, i, k);
+    if (k < 0 || k >= 65536) continue;
+    if (seen[k >> 6] >> (k & 63) & 1) return fail(OIVAE_E_ARG, "%s: index %d appears twice", who, k);
+    seen[k >> 6] |= (uint64_t)1 << (k & 63);
   }
   if (!workspace || !aligned_to(workspace, 8) || workspace_bytes < oivae_grad_norm_workspace_bytes(count))
     return fail(OIVAE_E_WORKSPACE, "%s: workspace of %lld bytes (8-byte aligned) needed", who,
@@ -599,10 +606,11 @@ static int check_grads(const char* who, const oivae_grad_t* t, int32_t count, vo
   return OIVAE_OK;
 }
 
-// the partial sums of all launches, one behind the other; their number into `parts`
+// the partial sums of all launches, one behind the other; their number into `parts`, that of the chunks into `chunks`
 static int launch_partials(const char* who, const oivae_grad_t* t, int32_t count, double* part, int64_t room, int64_t* parts,
-                           hipStream_t st) {
+                           int64_t* chunks, hipStream_t st) {
   *parts = 0;
+  *chunks = 0;
   return for_grad_launches(t, count, [&](const GradLaunch& a) -> int {
     if (a.chunks == 0) return OIVAE_OK;
     const unsigned blocks = a.chunks < (uint32_t)kNormBlocks ? a.chunks : (unsigned)kNormBlocks;
@@ -610,6 +618,7 @@ static int launch_partials(const char* who, const oivae_grad_t* t, int32_t count
     hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(kThreads), 0, st, a, part + *parts);
     OIVAE_LAUNCH_CHECK();
     *parts += blocks;
+    *chunks += a.chunks;
     return OIVAE_OK;
   });
 }
@@ -624,6 +633,7 @@ static int run_adamw(const char* who, bool eight, const oivae_adamw_tensor_t* t,
   if (!st->m || !st->v || (eight && (!st->m_scale || !st->v_scale))) return fail(OIVAE_E_ARG, "%s: null moment buffer", who);
   if (!aligned_to(st->m, 16) || !aligned_to(st->v, 16) || !aligned_to(st->master, 16))
     return fail(OIVAE_E_ARG, "%s: moment and master buffers must be 16-byte aligned", who);
+  int64_t place = 0;
   for (int32_t i = 0; i < count; ++i) {
     if (int rc = check_grad(who, i, t[i].g, t[i].n, t[i].g_type)) return rc;
     if (t[i].p_type < OIVAE_F32 || t[i].p_type > OIVAE_F16) return fail(OIVAE_E_ARG, "%s: tensor %d has unknown type %d", who, i, t[i].p_type);
@@ -632,6 +642,8 @@ static int run_adamw(const char* who, bool eight, const oivae_adamw_tensor_t* t,
     if (t[i].p_type != OIVAE_F32 && !st->master) return fail(OIVAE_E_ARG, "%s: half-precision parameters need master weights", who);
     if (t[i].at < 0 || t[i].at % kMomentBlock != 0 || t[i].at / kMomentBlock > (int64_t)0xFFFFFFFFu)
       return fail(OIVAE_E_ARG, "%s: tensor %d's place in the moment buffers must be a multiple of %d", who, i, kMomentBlock);
+    if (t[i].at < place) return fail(OIVAE_E_ARG, "%s: tensor %d's place in the moment buffers reaches into the one before it", who, i);
+    place = t[i].at + t[i].n;
     if (t[i].group < 0 || t[i].group >= n_groups) return fail(OIVAE_E_ARG, "%s: tensor %d names group %d of %d", who, i, t[i].group, n_groups);
     if (t[i].index < 0) return fail(OIVAE_E_ARG, "%s: tensor %d has a negative index", who, i);
     if (!st->steps && t[i].step < 1) return fail(OIVAE_E_ARG, "%s: tensor %d is at step %d", who, i, t[i].step);
@@ -724,9 +736,9 @@ extern "C" int oivae_grad_norm(const oivae_grad_t* grads, int32_t count, int32_t
       OIVAE_LAUNCH_CHECK();
       return OIVAE_OK;
     });
-  int64_t parts = 0;
+  int64_t parts = 0, all = 0;
   if (with_norm)
-    if (int rc = launch_partials(who, grads, count, part, workspace_bytes / (int64_t)sizeof(double), &parts, st)) return rc;
+    if (int rc = launch_partials(who, grads, count, part, workspace_bytes / (int64_t)sizeof(double), &parts, &all, st)) return rc;
   bool first = true;
   auto conclude_launch = [&](const GradLaunch& a) -> int {
     if (!first && !steps) return OIVAE_OK;
@@ -750,10 +762,10 @@ extern "C" int oivae_clip_grad_norm(const oivae_grad_t* grads, int32_t count, fl
   hipStream_t st = (hipStream_t)stream;
   if (int rc = poll_error_word(who, st)) return rc;
   double* part = static_cast<double*>(workspace);
-  int64_t parts = 0;
-  if (int rc = launch_partials(who, grads, count, part, workspace_bytes / (int64_t)sizeof(double), &parts, st)) return rc;
+  int64_t parts = 0, chunks = 0;
+  if (int rc = launch_partials(who, grads, count, part, workspace_bytes / (int64_t)sizeof(double), &parts, &chunks, st)) return rc;
   const bool scale = max_norm > 0.f && parts > 0;
-  const bool few = scale && parts <= kFewBlocks;
+  const bool few = scale && chunks <= kFewChunks;
   if (!few) {
     hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, st, (const double*)part, (int)parts, norm);
     OIVAE_LAUNCH_CHECK();

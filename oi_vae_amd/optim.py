@@ -315,6 +315,9 @@ class AdamW(_EngineOptimizer):
     for p in leaves:
       if not _dense(p):
         raise ValueError("a parameter of strides %s and shape %s does not fill its memory" % (p.stride(), tuple(p.shape)))
+    spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in leaves if p.numel())
+    if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+      raise ValueError("two parameters share memory")
     self._leaves, self.device = leaves, device
     self._lib = _lib.init_device(device.index)
     self._kinds = []

@@ -42,7 +42,7 @@ def test_record_sizes_are_those_of_the_header(tmp_path):
 @pytest.mark.parametrize("kw,word", [
   (dict(n=-1), "negative size"), (dict(g=0), "null gradient"), (dict(p=0), "is null"), (dict(g=8193, g_type=1), "aligned"),
   (dict(g=8194), "aligned"), (dict(p=4098), "aligned"), (dict(p_type=3), "unknown type"), (dict(g_type=-1), "unknown gradient"),
-  (dict(p_type=1), "master"), (dict(at=64), "multiple of 128"), (dict(at=-128), "multiple of 128"), (dict(group=1), "group"),
+  (dict(p_type=1), "master"), (dict(at=64), "multiple of 128"), (dict(at=128), "reaches into"), (dict(at=0), "reaches into"), (dict(at=-128), "multiple of 128"), (dict(group=1), "group"),
   (dict(group=-1), "group"), (dict(index=-1), "index"), (dict(step=0), "step"), (dict(n=(1 << 40) + 1), "elements")])
 def test_entry_points_refuse_bad_tensors(kw, word):
   from oi_vae_amd import optim
@@ -72,7 +72,7 @@ def test_entry_points_refuse_bad_calls():
   assert call(st=lib.AdamwState(1 << 20, (2 << 20) + 8, None, None, None, None)) == 1
   assert call(st=lib.AdamwState(1 << 20, 2 << 20, None, None, None, None), eight=True) == 1     # no scales
   g = np.zeros(2, optim._GRAD)
-  g["g"], g["n"] = 4096, 10
+  g["g"], g["n"], g["index"] = 4096, 10, [0, 1]
   need = L.oivae_grad_norm_workspace_bytes(2)
   norm = lambda clip=1 << 20, steps=None, b1=0.9, ws=2 << 20, nb=need, count=2, rec=g.ctypes.data: L.oivae_grad_norm(
     rec, count, 1, 1.0, 1.0, clip, steps, b1, 0.999, ws, nb, None)
@@ -84,6 +84,8 @@ def test_entry_points_refuse_bad_calls():
     keep, g[field][1] = g[field][1], bad
     assert norm() == 1 and scale() == 1, (field, bad)
     g[field][1] = keep
+  g["index"] = 5
+  assert norm() == 1 and b"twice" in L.oivae_last_error() and scale() == 1
   assert L.oivae_grad_norm_workspace_bytes(0) >= 8 and L.oivae_grad_norm_workspace_bytes(10000) > need
 
 

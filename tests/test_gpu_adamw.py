@@ -667,6 +667,10 @@ def test_refusals_at_the_first_step():
     opt.step()
   with pytest.raises(ValueError, match="more than once"):
     optim.clip_grad_norm_([q, q], 1.0)
+  flat = torch.zeros(100, device="cuda")
+  with pytest.raises(ValueError, match="share memory"):
+    optim.AdamW([flat[:50].detach().requires_grad_(), flat[49:].detach().requires_grad_()]).buffers
+  optim.AdamW([flat[:50].detach().requires_grad_(), flat[50:].detach().requires_grad_()]).buffers
   with pytest.raises(RuntimeError, match="max_grad_norm"):
     opt.grad_norm
   other = optim.AdamW([torch.zeros(9, device="cuda").requires_grad_()], state_bits=8)
