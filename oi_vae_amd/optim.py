@@ -229,7 +229,8 @@ class AdamW(_EngineOptimizer):
 
   Two uses: handed to `OIVAE(optimizers=[AdamW(...), SGD(...)])` it steps the engine's flat buffers in place of `Adam` (one
   lr, weight_decay and state_bits for all groups); by itself it steps the `.grad` of any float32, bfloat16 or float16
-  tensors on one GPU.  Per group: `lr`, `weight_decay`, `state_bits`; `betas` and `eps` are one for all.
+  tensors on one GPU.  Per group: `lr`, `weight_decay`, `state_bits` (the last fixed at first use, as the parameters are);
+  `betas` and `eps` are one for all.
 
   state_bits=8 holds both moments in 8 bits: blocks of 128 elements of a tensor share a power of two; first moments are
   e4m3 codes, second moments e5m2 codes, rounded stochastically with bits drawn from (seed, step, tensor, element) -- two
@@ -406,12 +407,14 @@ class AdamW(_EngineOptimizer):
 
   def state_dict(self):
     """Everything a resumed run needs: counts, options and copies of `buffers`."""
-    return {"steps": self.steps(), "seed": self.seed,
+    self.buffers
+    return {"steps": self.steps(), "seed": self.seed, "sizes": [p.numel() for p in self._leaves],
             "groups": [{k: v.clone() if torch.is_tensor(v) else v for k, v in g.items() if k != "params"} for g in self.param_groups],
             "buffers": {bits: {k: t.clone() for k, t in held.items()} for bits, held in self.buffers.items()}}
 
   @torch.no_grad()
   def load_state_dict(self, state):
+    """Takes over a state_dict of an AdamW over parameters of the same sizes, types and groups; all or nothing."""
     held = self.buffers
     for what, mine, theirs in [("bits", held, state["buffers"])] + [("buffers", held[b], state["buffers"].get(b, {})) for b in held]:
       if sorted(mine) != sorted(theirs):
@@ -420,15 +423,14 @@ class AdamW(_EngineOptimizer):
     for t, src, k in pairs:
       if src.shape != t.shape or src.dtype != t.dtype:
         raise ValueError("%s is %s %s in the state, %s %s here" % (k, tuple(src.shape), src.dtype, tuple(t.shape), t.dtype))
-    if len(state["groups"]) != len(self.param_groups) or len(state["steps"]) != len(self._leaves):
-      raise ValueError("the state was made for other parameter groups")
+    if (list(state["sizes"]) != [p.numel() for p in self._leaves] or len(state["groups"]) != len(self.param_groups)
+        or any(src["state_bits"] != g["state_bits"] for src, g in zip(state["groups"], self.param_groups))):
+      raise ValueError("the state was made for other parameters or groups")
     for t, src, _ in pairs:
       t.view(torch.uint8).copy_(src.view(torch.uint8))
     self.set_steps(state["steps"])
     self.seed = state["seed"]
     for g, src in zip(self.param_groups, state["groups"]):
-      if any(src[k] != g[k] for k in ("state_bits",)):
-        raise ValueError("the state holds other state_bits")
       for k, v in src.items():
         if torch.is_tensor(g[k]):
           g[k].copy_(torch.as_tensor(v))     # an lr on the device stays where a captured graph reads it

@@ -673,9 +673,15 @@ def test_refusals_at_the_first_step():
   optim.AdamW([flat[:50].detach().requires_grad_(), flat[50:].detach().requires_grad_()]).buffers
   with pytest.raises(RuntimeError, match="max_grad_norm"):
     opt.grad_norm
-  other = optim.AdamW([torch.zeros(9, device="cuda").requires_grad_()], state_bits=8)
-  with pytest.raises(ValueError, match="bits"):
-    other.load_state_dict(opt.state_dict())
+  make = lambda sizes, **kw: optim.AdamW([torch.zeros(n, device="cuda").requires_grad_() for n in sizes], **kw)
+  state = make([9, 200]).state_dict()
+  for other, what in ((make([9, 200], state_bits=8), "bits"), (make([9]), "exp_avg"), (make([8, 201]), "other parameters"),
+                      (make([200, 9]), "other parameters")):
+    keep = {b: {k: t.view(torch.uint8).clone() for k, t in held.items()} for b, held in other.buffers.items()}
+    with pytest.raises(ValueError, match=what):
+      other.load_state_dict(state)
+    assert all(torch.equal(t.view(torch.uint8), keep[b][k]) for b, held in other.buffers.items() for k, t in held.items())
+  make([9, 200]).load_state_dict(state)
 
 
 # ---- together, and in the framework's own training step --------------------------------------------------------------------
