@@ -151,6 +151,11 @@ def _lists():
 _lists_module = None
 
 
+def _stream(index):
+  """Handle of the current stream of a device (torch.cuda.current_stream builds a Stream object first, for 1 us)."""
+  return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _written(t):
   """Tells autograd that a kernel writes t."""
   if not t.is_inference():
@@ -190,7 +195,7 @@ def _clip(got, max_norm):
   # norm and workspace of this call alone: calls on other streams and in captured graphs have their own
   norm, ws = torch.empty((), device="cuda"), torch.empty(nbytes, dtype=torch.uint8, device="cuda")
   _lib.check(L.oivae_clip_grad_norm(address, count, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes,
-                                    torch.cuda.current_stream(device).cuda_stream), "oivae_clip_grad_norm")
+                                    _stream(device)), "oivae_clip_grad_norm")
   return norm
 
 
@@ -514,7 +519,7 @@ class AdamW(_EngineOptimizer):
       todo.append((k, rec))
     if partial and not any(len(rec) for _, rec in todo):
       return
-    stream = torch.cuda.current_stream(index).cuda_stream
+    stream = _stream(index)
     clip = None
     if self._on_device:
       clip = self._clip.data_ptr()
