@@ -496,7 +496,7 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
 // 32 lanes hold one block, four elements each (one vector per thread and stream, as above).  With 16 lanes and 8 elements
 // a lane the vectors of a wave are 32 bytes apart: 861 us on 268M bf16 parameters against 719.
 //   kFast: hardware root and reciprocal (one unit in the last place each) instead of the correctly rounded ones, about a
-// third of the instructions: 719 against 779 us (706 now, 6.1 TB/s).  The hardware root takes subnormals for zero: up to
+// third of the instructions: 719 against 779 us (694 now, 6.2 TB/s).  The hardware root takes subnormals for zero: up to
 // 1.1e-19, times 1 / sqrt(1 - b2) at most, in a denominator of at least eps.
 template <bool kFast>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(AdamwLaunch a) {
