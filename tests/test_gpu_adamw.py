@@ -199,6 +199,27 @@ def test_groups_with_options_of_their_own():
   _check(opt, before, _state(opt), grads, 7, [1e-3 * (k + 1) for k in range(len(ps))], [0.01 * k for k in range(len(ps))])
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_of_another_type_than_their_parameter(bits):
+  """float32 gradients of 16-bit parameters (accumulated there) and the reverse, in one list, with clipping behind it."""
+  from oi_vae_amd import optim
+  ps = _params([300, 4097], torch.bfloat16, seed=3) + _params([129, 7], torch.float32, seed=4) + _params([1000], torch.float16, seed=5)
+  for p, typ in zip(ps, (torch.float32, torch.float16, torch.bfloat16, torch.float16, torch.float32)):
+    g = p.grad.to(typ)
+    p.grad = None
+    p.grad_dtype = typ
+    p.grad = g
+  opt = _opt(ps, 6, lr=1e-3, weight_decay=0.1, state_bits=bits)
+  before, grads = _state(opt), [_np(p.grad) for p in ps]
+  opt.step()
+  _check(opt, before, _state(opt), grads, 6, [1e-3] * 5, [0.1] * 5)
+  norm = np.sqrt(sum((g * g).sum() for g in grads))
+  assert abs(optim.clip_grad_norm_(ps, norm / 3).item() - norm) <= 2 * U * norm
+  for p, g in zip(ps, grads):
+    eps = torch.finfo(p.grad.dtype).eps / 2
+    assert np.all(np.abs(_np(p.grad) - g / 3) <= (eps + 8 * U) * np.abs(g / 3) + 1e-6 / norm * np.abs(g) + 2.0 ** -25)
+
+
 @pytest.mark.parametrize("on_device", [False, True])
 def test_parameters_without_a_gradient_wait(on_device):
   ps = _params([50, 60, 70], torch.float32, seed=1)
