@@ -269,13 +269,14 @@ int oivae_adam_f32(float* p, const float* g, float* m, float* v, int64_t n,
  * The tensor lists are HOST arrays, read during the call; nothing is uploaded and no pointer is kept.
  * A tensor is dense memory of n elements (any alignment that its element type allows); gradient and parameter share the
  * order of their elements.  Parameters of 16 bits are rounded copies (to nearest) of fp32 master weights. */
-enum { OIVAE_F32 = 0, OIVAE_BF16 = 1, OIVAE_F16 = 2 };
+enum { OIVAE_F32 = 0, OIVAE_BF16 = 1, OIVAE_F16 = 2, OIVAE_F32_WATCHED = 3 };
 #define OIVAE_ADAMW_BLOCK 128   /* a tensor's place in the moment buffers is a whole number of these blocks */
 
 typedef struct {
   void* g;          /* device */
   int64_t n;
-  int32_t type;     /* OIVAE_F32 | OIVAE_BF16 | OIVAE_F16 */
+  int32_t type;     /* OIVAE_F32 | OIVAE_BF16 | OIVAE_F16; oivae_grad_norm also takes OIVAE_F32_WATCHED: floats that do not
+                       enter the norm, but have to be finite for it to be so */
   int32_t index;    /* of its step counter; -1: none */
 } oivae_grad_t;
 
@@ -339,6 +340,11 @@ int oivae_grad_norm(const oivae_grad_t* grads, int32_t count, int32_t with_norm,
 /* Norm into *norm (device), then g *= coef in place (max_norm <= 0, or a coefficient of 1: nothing is touched). */
 int oivae_clip_grad_norm(const oivae_grad_t* grads, int32_t count, float max_norm, float* norm, void* workspace,
                          int64_t workspace_bytes, void* stream);
+
+/* oivae_sgd_prox_f32 behind an AdamW step of the other parameters: Ws, zero_mask and row_norms stay as they are where the
+ * verdict `clip` (may be NULL), from oivae_grad_norm on the same stream, leaves the step out. */
+int oivae_sgd_prox_clip_f32(float* Ws, const float* dWs, int64_t rows, int32_t H, float lr, float t, int32_t do_prox,
+                            uint8_t* zero_mask, float* row_norms, const oivae_clip_t* clip, void* stream);
 
 /* One AdamW step of `count` tensors; `clip` (may be NULL) from oivae_grad_norm on the same stream. */
 int oivae_adamw_f32(const oivae_adamw_tensor_t* tensors, int32_t count, const oivae_adamw_group_t* groups, int32_t n_groups,

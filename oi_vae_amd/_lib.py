@@ -26,9 +26,10 @@ SYMBOLS = [
   "oivae_check_errors", "oivae_small_step_applies", "oivae_small_step_f32",
   "oivae_gamma_workspace_bytes", "oivae_gamma_logprob_f32",
   "oivae_grad_norm_workspace_bytes", "oivae_grad_norm", "oivae_clip_grad_norm", "oivae_adamw_f32", "oivae_adamw_f8",
+  "oivae_sgd_prox_clip_f32",
 ]
 
-F32, BF16, F16 = 0, 1, 2     # element types of the optimizer operators over lists of tensors
+F32, BF16, F16, F32_WATCHED = 0, 1, 2, 3     # element types of the optimizer operators over lists of tensors
 ADAMW_BLOCK = 128            # OIVAE_ADAMW_BLOCK
 
 
@@ -111,7 +112,8 @@ def bind(path):
                                 ctypes.c_double, c_f, c_vp, c_vp]
   L.oivae_adamw_f8.argtypes = [c_vp, c_i32, c_vp, c_i32, ctypes.POINTER(AdamwState), ctypes.c_double, ctypes.c_double,
                                ctypes.c_double, c_f, ctypes.c_uint32, c_vp, c_vp]
-  for name in ("oivae_grad_norm", "oivae_clip_grad_norm", "oivae_adamw_f32", "oivae_adamw_f8"):
+  L.oivae_sgd_prox_clip_f32.argtypes = [c_vp, c_vp, c_i64, c_i32, c_f, c_f, c_i32, c_vp, c_vp, c_vp, c_vp]
+  for name in ("oivae_grad_norm", "oivae_clip_grad_norm", "oivae_adamw_f32", "oivae_adamw_f8", "oivae_sgd_prox_clip_f32"):
     getattr(L, name).restype = ctypes.c_int
   L.oivae_reload_test_hooks.argtypes = []
   L.oivae_reload_test_hooks.restype = None

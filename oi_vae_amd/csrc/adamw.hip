@@ -140,7 +140,7 @@ struct GradLaunch {
 };
 
 // elements of one chunk: 256 threads x four vectors of 16 bytes
-__host__ __device__ inline int grad_chunk(int type) { return type == OIVAE_F32 ? 4096 : 8192; }
+__host__ __device__ inline int grad_chunk(int type) { return type == OIVAE_F32 || type == OIVAE_F32_WATCHED ? 4096 : 8192; }
 
 // The last slot whose first chunk is not behind `chunk`, by bisection over scalar loads; the first chunks lie side by side, a few
 // cache lines (within the slots: 0.7 us more of a 5 us launch).  A ballot over the lanes' comparisons saves 0.3 us there and
@@ -192,14 +192,21 @@ __device__ __forceinline__ double sum_of_squares(const GradLaunch& a) {
     const GradSlot& s = a.s[k];
     const int type = a.info[k] & 3;
     const int64_t base = (int64_t)(c - a.first[k]) * grad_chunk(type);
-    if (type == OIVAE_F32) {
+    if (type == OIVAE_F32 || type == OIVAE_F32_WATCHED) {
       f4 x[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) x[u] = load4(s.g, OIVAE_F32, base + (u * kThreads + threadIdx.x) * 4, s.n);
+      if (type == OIVAE_F32_WATCHED) {   // zeros, which change no sum, or NaN where an element is not finite
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j & 1] = fma((double)x[u][j], (double)x[u][j], acc[j & 1]);
+          for (int j = 0; j < 4; ++j) acc[j & 1] += (double)(x[u][j] * 0.f);
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j & 1] = fma((double)x[u][j], (double)x[u][j], acc[j & 1]);
+      }
     } else {
       h8 h[4];
 #pragma unroll
@@ -559,14 +566,14 @@ __global__ __launch_bounds__(kThreads) void adamw8_kernel(AdamwLaunch a) {
 
 // ---- host --------------------------------------------------------------------------------------------------------------
 static bool aligned_to(const void* p, int a) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(a - 1)) == 0; }
-static int size_of(int type) { return type == OIVAE_F32 ? 4 : 2; }
+static int size_of(int type) { return type == OIVAE_F32 || type == OIVAE_F32_WATCHED ? 4 : 2; }
 
 constexpr uint32_t kMaxChunks = 0xFFFFFFu;   // workgroups of one launch: a grid's size in threads stays below 2^32
 constexpr int64_t kMaxElements = (int64_t)kMaxChunks * kChunk;   // of one tensor
 
-static int check_grad(const char* who, int32_t i, const void* g, int64_t n, int32_t type) {
+static int check_grad(const char* who, int32_t i, const void* g, int64_t n, int32_t type, int32_t last_type = OIVAE_F16) {
   if (n < 0) return fail(OIVAE_E_ARG, "%s: tensor %d has a negative size", who, i);
-  if (type < OIVAE_F32 || type > OIVAE_F16) return fail(OIVAE_E_ARG, "%s: tensor %d has unknown gradient type %d", who, i, type);
+  if (type < OIVAE_F32 || type > last_type) return fail(OIVAE_E_ARG, "%s: tensor %d has unknown gradient type %d", who, i, type);
   if (n > 0 && !g) return fail(OIVAE_E_ARG, "%s: tensor %d has a null gradient", who, i);
   if (!aligned_to(g, size_of(type))) return fail(OIVAE_E_ARG, "%s: gradient %d is not aligned to its elements", who, i);
   if (n > kMaxElements) return fail(OIVAE_E_SHAPE, "%s: tensor %d has more than %lld elements", who, i, (long long)kMaxElements);
@@ -596,10 +603,11 @@ static int for_grad_launches(const oivae_grad_t* t, int32_t count, F&& launch) {
   return a.count > 0 ? launch(a) : OIVAE_OK;
 }
 
-static int check_grads(const char* who, const oivae_grad_t* t, int32_t count, void* workspace, int64_t workspace_bytes) {
+static int check_grads(const char* who, const oivae_grad_t* t, int32_t count, void* workspace, int64_t workspace_bytes,
+                       int32_t last_type) {
   uint64_t seen[1024] = {0};   // indices below 65536: two threads would advance a counter named twice
   for (int32_t i = 0; i < count; ++i) {
-    if (int rc = check_grad(who, i, t[i].g, t[i].n, t[i].type)) return rc;
+    if (int rc = check_grad(who, i, t[i].g, t[i].n, t[i].type, last_type)) return rc;
     const int32_t k = t[i].index;
     if (k < -1 || k >= 1 << 29) return fail(OIVAE_E_ARG, "%s: tensor %d has index %d", who, i, k);
     if (k < 0 || k >= 65536) continue;
@@ -725,7 +733,7 @@ extern "C" int oivae_grad_norm(const oivae_grad_t* grads, int32_t count, int32_t
   if (count < 0 || (count > 0 && !grads) || !clip) return fail(OIVAE_E_ARG, "%s: bad argument", who);
   if (steps && !(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0))
     return fail(OIVAE_E_ARG, "%s: betas must be in [0, 1)", who);
-  if (int rc = check_grads(who, grads, count, workspace, workspace_bytes)) return rc;
+  if (int rc = check_grads(who, grads, count, workspace, workspace_bytes, OIVAE_F32_WATCHED)) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (int rc = poll_error_word(who, st)) return rc;
   double* part = static_cast<double*>(workspace);
@@ -765,7 +773,7 @@ extern "C" int oivae_clip_grad_norm(const oivae_grad_t* grads, int32_t count, fl
                                     int64_t workspace_bytes, void* stream) {
   const char* who = "oivae_clip_grad_norm";
   if (count < 0 || (count > 0 && !grads) || !norm) return fail(OIVAE_E_ARG, "%s: bad argument", who);
-  if (int rc = check_grads(who, grads, count, workspace, workspace_bytes)) return rc;
+  if (int rc = check_grads(who, grads, count, workspace, workspace_bytes, OIVAE_F16)) return rc;
   hipStream_t st = (hipStream_t)stream;
   if (int rc = poll_error_word(who, st)) return rc;
   double* part = static_cast<double*>(workspace);

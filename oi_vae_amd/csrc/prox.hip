@@ -18,6 +18,13 @@
 
 namespace oivae {
 
+// Whether the step that this launch belongs to changes nothing: a decoder launch of it failed (common.h ErrWords), or the
+// verdict on its gradients (oivae_grad_norm) leaves it out -- the whole step, Ws among the rest: one step with a NaN in its
+// gradients would otherwise reach Ws, and through it every gradient of every later step.
+__device__ __forceinline__ bool left_out(const uint16_t* __restrict__ tab, const oivae_clip_t* __restrict__ clip) {
+  return *reinterpret_cast<const uint32_t*>(tab + kBadWordOffsetU16) != 0 || (clip != nullptr && clip->skip != 0);
+}
+
 // ---- path A: any H, one thread per row, scalar emulation of the sum order ----
 template <bool SGD>
 __global__ __launch_bounds__(256) void prox_rows_scalar(float* __restrict__ Ws,
@@ -26,8 +33,9 @@ __global__ __launch_bounds__(256) void prox_rows_scalar(float* __restrict__ Ws,
                                                         int do_prox,
                                                         uint8_t* __restrict__ mask,
                                                         float* __restrict__ norms,
-                                                        const uint16_t* __restrict__ tab) {
-  if (*reinterpret_cast<const uint32_t*>(tab + kBadWordOffsetU16) != 0) return;   // a decoder launch of this step failed: no update (common.h ErrWords)
+                                                        const uint16_t* __restrict__ tab,
+                                                        const oivae_clip_t* __restrict__ clip) {
+  if (left_out(tab, clip)) return;
   const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (r >= rows) return;
   prox_row_scalar_dev<SGD>(Ws, dWs, r, H, neg_lr, t, do_prox, mask, norms, tab);
@@ -101,8 +109,9 @@ __global__ __launch_bounds__(256) void prox_rows_vec(float* __restrict__ Ws,
                                                      int64_t rows, float neg_lr, float t, int do_prox,
                                                      uint8_t* __restrict__ mask,
                                                      float* __restrict__ norms,
-                                                     const uint16_t* __restrict__ tab) {
-  if (*reinterpret_cast<const uint32_t*>(tab + kBadWordOffsetU16) != 0) return;   // a decoder launch of this step failed: no update (common.h ErrWords)
+                                                     const uint16_t* __restrict__ tab,
+                                                     const oivae_clip_t* __restrict__ clip) {
+  if (left_out(tab, clip)) return;
   constexpr int H = 8 * V;
   const int64_t gt = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t r = gt >> 1;
@@ -151,8 +160,9 @@ __global__ __launch_bounds__(kProxLdsThreads, 1) void prox_rows_vec_lds(float* _
                                                                         int64_t rows, float neg_lr, float t, int do_prox,
                                                                         uint8_t* __restrict__ mask,
                                                                         float* __restrict__ norms,
-                                                                        const uint16_t* __restrict__ tab) {
-  if (*reinterpret_cast<const uint32_t*>(tab + kBadWordOffsetU16) != 0) return;   // a decoder launch of this step failed: no update (common.h ErrWords)
+                                                                        const uint16_t* __restrict__ tab,
+                                                                        const oivae_clip_t* __restrict__ clip) {
+  if (left_out(tab, clip)) return;
   constexpr int H = 8 * V;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   uint16_t* ltab = reinterpret_cast<uint16_t*>(smem_raw);   // [65536]
@@ -214,8 +224,9 @@ template <bool SGD>
 __global__ __launch_bounds__(256) void prox_rows_wide(float* __restrict__ Ws, const float* __restrict__ dWs,
                                                       int64_t rows, int H, float neg_lr, float t, int do_prox,
                                                       uint8_t* __restrict__ mask, float* __restrict__ norms,
-                                                      const uint16_t* __restrict__ tab) {
-  if (*reinterpret_cast<const uint32_t*>(tab + kBadWordOffsetU16) != 0) return;   // a decoder launch of this step failed: no update (common.h ErrWords)
+                                                      const uint16_t* __restrict__ tab,
+                                                      const oivae_clip_t* __restrict__ clip) {
+  if (left_out(tab, clip)) return;
   const int sub = threadIdx.x & 31;                                    // chain: accumulator k = sub / 8, lane l = sub % 8
   const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const bool live = r < rows;                                           // uniform per group of 32
@@ -364,7 +375,7 @@ __global__ __launch_bounds__(256) void prox_cols(float* __restrict__ W, const in
 
 template <int VV, bool SGD>
 static int launch_prox_vec(float* Ws, const float* dWs, int64_t rows, float neg_lr, float t, int do_prox, uint8_t* mask,
-                           float* norms, const uint16_t* tab, hipStream_t st) {
+                           float* norms, const uint16_t* tab, const oivae_clip_t* clip, hipStream_t st) {
   // path C from 4 passes of 256 workgroups up (512 rows each per pass), for rows of at most 128 bytes (two rows per
   // thread in registers under 1024 threads per workgroup; at 256 bytes the fused-SGD form spills)
   if constexpr (VV <= 4) {
@@ -372,19 +383,19 @@ static int launch_prox_vec(float* Ws, const float* dWs, int64_t rows, float neg_
       OIVAE_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&prox_rows_vec_lds<VV, SGD>),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, 131072));
       hipLaunchKernelGGL((prox_rows_vec_lds<VV, SGD>), dim3(256), dim3(kProxLdsThreads), 131072, st, Ws, dWs, rows,
-                         neg_lr, t, do_prox, mask, norms, tab);
+                         neg_lr, t, do_prox, mask, norms, tab, clip);
       return OIVAE_OK;
     }
   }
   const unsigned blocks = (unsigned)((rows * 2 + 255) / 256);
   hipLaunchKernelGGL((prox_rows_vec<VV, SGD>), dim3(blocks), dim3(256), 0, st, Ws, dWs, rows, neg_lr, t, do_prox, mask,
-                     norms, tab);
+                     norms, tab, clip);
   return OIVAE_OK;
 }
 
 template <bool SGD>
 static int launch_prox(float* Ws, const float* dWs, int64_t rows, int H, float lr, float t,
-                       int do_prox, uint8_t* mask, float* norms, hipStream_t st) {
+                       int do_prox, uint8_t* mask, float* norms, const oivae_clip_t* clip, hipStream_t st) {
   const uint16_t* tab = rsqrt14_table_device();
   if (!tab) return fail(OIVAE_E_NOINIT, "oivae_init has not been called on this device");
   if (rows == 0) return OIVAE_OK;
@@ -392,7 +403,7 @@ static int launch_prox(float* Ws, const float* dWs, int64_t rows, int H, float l
   const bool aligned = ((reinterpret_cast<uintptr_t>(Ws) & 15) == 0) &&
                        (!SGD || (reinterpret_cast<uintptr_t>(dWs) & 15) == 0);
 #define OIVAE_PROX_VEC(VV)                                                                        \
-  { if (int rc = launch_prox_vec<VV, SGD>(Ws, dWs, rows, neg_lr, t, do_prox, mask, norms, tab, st)) return rc; }
+  { if (int rc = launch_prox_vec<VV, SGD>(Ws, dWs, rows, neg_lr, t, do_prox, mask, norms, tab, clip, st)) return rc; }
   if (aligned && H == 8) OIVAE_PROX_VEC(1)
   else if (aligned && H == 16) OIVAE_PROX_VEC(2)
   else if (aligned && H == 32) OIVAE_PROX_VEC(4)
@@ -401,11 +412,11 @@ static int launch_prox(float* Ws, const float* dWs, int64_t rows, int H, float l
   else if (H >= 512) {
     const unsigned blocks = (unsigned)((rows * 32 + 255) / 256);
     hipLaunchKernelGGL((prox_rows_wide<SGD>), dim3(blocks), dim3(256), 0, st, Ws, dWs, rows, H,
-                       neg_lr, t, do_prox, mask, norms, tab);
+                       neg_lr, t, do_prox, mask, norms, tab, clip);
   } else {
     const unsigned blocks = (unsigned)((rows + 255) / 256);
     hipLaunchKernelGGL((prox_rows_scalar<SGD>), dim3(blocks), dim3(256), 0, st, Ws, dWs, rows, H,
-                       neg_lr, t, do_prox, mask, norms, tab);
+                       neg_lr, t, do_prox, mask, norms, tab, clip);
   }
 #undef OIVAE_PROX_VEC
   OIVAE_LAUNCH_CHECK();
@@ -423,18 +434,28 @@ extern "C" int oivae_prox_f32(float* Ws, int64_t rows, int32_t H, float t, uint8
     return fail(OIVAE_E_SHAPE, "oivae_prox_f32: H=%d outside [1, 2^20] (the reference's row-sum order is pinned only there)", H);
   if (rows * 2 / 256 > 0x7fffffffLL) return fail(OIVAE_E_SHAPE, "oivae_prox_f32: too many rows");
   if (int rc = poll_error_word("oivae_prox_f32", (hipStream_t)stream)) return rc;
-  return launch_prox<false>(Ws, nullptr, rows, H, 0.f, t, 1, zero_mask, row_norms, (hipStream_t)stream);
+  return launch_prox<false>(Ws, nullptr, rows, H, 0.f, t, 1, zero_mask, row_norms, nullptr, (hipStream_t)stream);
+}
+
+static int sgd_prox(const char* who, float* Ws, const float* dWs, int64_t rows, int32_t H, float lr, float t, int32_t do_prox,
+                    uint8_t* zero_mask, float* row_norms, const oivae_clip_t* clip, hipStream_t st) {
+  if (!Ws || !dWs || rows < 0) return fail(OIVAE_E_ARG, "%s: null pointer or negative rows", who);
+  if (H < 1 || H > (1 << 20)) return fail(OIVAE_E_SHAPE, "%s: H=%d outside [1, 2^20]", who, H);
+  if (rows * 2 / 256 > 0x7fffffffLL) return fail(OIVAE_E_SHAPE, "%s: too many rows", who);
+  if (int rc = poll_error_word(who, st)) return rc;
+  return launch_prox<true>(Ws, dWs, rows, H, lr, t, do_prox ? 1 : 0, zero_mask, row_norms, clip, st);
 }
 
 extern "C" int oivae_sgd_prox_f32(float* Ws, const float* dWs, int64_t rows, int32_t H, float lr,
                                   float t, int32_t do_prox, uint8_t* zero_mask, float* row_norms,
                                   void* stream) {
-  if (!Ws || !dWs || rows < 0) return fail(OIVAE_E_ARG, "oivae_sgd_prox_f32: null pointer or negative rows");
-  if (H < 1 || H > (1 << 20))
-    return fail(OIVAE_E_SHAPE, "oivae_sgd_prox_f32: H=%d outside [1, 2^20]", H);
-  if (rows * 2 / 256 > 0x7fffffffLL) return fail(OIVAE_E_SHAPE, "oivae_sgd_prox_f32: too many rows");
-  if (int rc = poll_error_word("oivae_sgd_prox_f32", (hipStream_t)stream)) return rc;
-  return launch_prox<true>(Ws, dWs, rows, H, lr, t, do_prox ? 1 : 0, zero_mask, row_norms, (hipStream_t)stream);
+  return sgd_prox("oivae_sgd_prox_f32", Ws, dWs, rows, H, lr, t, do_prox, zero_mask, row_norms, nullptr, (hipStream_t)stream);
+}
+
+extern "C" int oivae_sgd_prox_clip_f32(float* Ws, const float* dWs, int64_t rows, int32_t H, float lr, float t,
+                                       int32_t do_prox, uint8_t* zero_mask, float* row_norms, const oivae_clip_t* clip,
+                                       void* stream) {
+  return sgd_prox("oivae_sgd_prox_clip_f32", Ws, dWs, rows, H, lr, t, do_prox, zero_mask, row_norms, clip, (hipStream_t)stream);
 }
 
 extern "C" int oivae_prox_cols_f32(float* W, const int32_t* group_off, int32_t G, int32_t K, int32_t max_group_rows,

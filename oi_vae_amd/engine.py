@@ -398,14 +398,15 @@ class Engine:
                                          self.zero_mask.data_ptr(), self.row_norms.data_ptr(), self._stream()),
                  "oivae_prox_f32")
 
-  def sgd_prox_step(self, lr: float, t: float, do_prox: bool = True):
-    """Ws -= lr*dWs then the proximal step, one kernel."""
+  def sgd_prox_step(self, lr: float, t: float, do_prox: bool = True, verdict=None):
+    """Ws -= lr*dWs then the proximal step, one kernel.  ``verdict``: the address of an oivae_clip_t (optim.AdamW's); where it
+    leaves the step out, Ws, zero_mask and row_norms stay as they are."""
     s = self.spec
     with torch.cuda.device(self.device):
-      _lib.check(self.lib.oivae_sgd_prox_f32(self.p["Ws"].data_ptr(), self.g["Ws"].data_ptr(), s.G * s.K, s.H,
-                                             float(lr), float(t), 1 if do_prox else 0,
-                                             self.zero_mask.data_ptr(), self.row_norms.data_ptr(), self._stream()),
-                 "oivae_sgd_prox_f32")
+      _lib.check(self.lib.oivae_sgd_prox_clip_f32(self.p["Ws"].data_ptr(), self.g["Ws"].data_ptr(), s.G * s.K, s.H,
+                                                  float(lr), float(t), 1 if do_prox else 0, self.zero_mask.data_ptr(),
+                                                  self.row_norms.data_ptr(), verdict, self._stream()),
+                 "oivae_sgd_prox_clip_f32")
 
   def adam_step(self, lr: float, betas=(0.9, 0.999), eps: float = 1e-8, grad_scale: float = 1.0, part=None):
     """torch.optim.Adam (default options) over every non-Ws parameter, one kernel.  ``part`` splits the update along

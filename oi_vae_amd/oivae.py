@@ -5,7 +5,7 @@ import torch
 from . import _lib, parallel
 from .adopt import adopt, probe_encoder_head
 from .distributions import Normal
-from .optim import Adam as _EngineAdam, SGD as _EngineSGD, _EngineOptimizer
+from .optim import Adam as _EngineAdam, AdamW as _EngineAdamW, SGD as _EngineSGD, _EngineOptimizer
 
 
 class NormalPriorTheta(object):
@@ -48,6 +48,7 @@ class OIVAE(object):
     self.engine = adopt(inference_model, generative_model, device=device)
     self._fused_sgd = None
     self._fused_adam = None
+    self._adamw = None
     self._foreign = []     # caller-owned torch.optim instances: (optimizer, [(parameter, its gradient view), ...])
     grad_of = {id(t): gv for t, gv in self.engine.bound}
     for opt in optimizers:
@@ -59,7 +60,9 @@ class OIVAE(object):
         if isinstance(opt, _EngineSGD):
           self._fused_sgd = opt
         elif isinstance(opt, _EngineAdam):
-          self._fused_adam = opt   # (AdamW steps the flat buffers by itself, after every gradient is final)
+          self._fused_adam = opt
+        elif isinstance(opt, _EngineAdamW):
+          self._adamw = opt        # steps the flat buffers by itself, after every gradient is final
       else:
         ps = [p for g in opt.param_groups for p in g["params"]]
         self._foreign.append((opt, [(p, grad_of[id(p)]) for p in ps if id(p) in grad_of]))
@@ -112,13 +115,10 @@ class OIVAE(object):
                                gen_sig_off=eng.gen_sig_off, prior_mu=pm, prior_sigma=ps,
                                sigma_theta=float(self.prior_theta.sigma), lam=float(self.lam), grad_sync=sync)
     scalars = out["scalars"].clone()
-    fuse = self._fused_sgd is not None and self.lam > 0
-    if self._fused_sgd is not None:
-      self._fused_sgd.fused_with_prox = fuse
     if dp and self._all_native:
       # bucket by bucket: the decoder-side gradients (reduced under the encoder backward GEMM) are final first, and
       # their Adam, SGD and proximal step run while the encoder bucket is still being reduced
-      a = self._fused_adam
+      a, fuse = self._fused_adam, self.lam > 0
       sync.wait_decoder()
       eng.adam_step(a._lr(), betas=a._uniform("betas"), eps=a._uniform("eps"), part="dec")
       eng.sgd_prox_step(self._fused_sgd._lr(), prox_step_size if fuse else 0.0, do_prox=fuse)
@@ -129,13 +129,23 @@ class OIVAE(object):
     if dp:
       sync.wait()
       parallel.reduce_scalars_(scalars, self.process_group)
+    self._update(prox_step_size)
+    return self._info(out, scalars)
+
+  def _update(self, prox_step_size):
+    """The optimizers on final gradients, the engine's SGD (with the proximal step) behind the others: it shares AdamW's
+    verdict, so that a step that is left out leaves Ws alone too."""
+    fuse = self.lam > 0
+    if self._fused_sgd is not None:
+      self._fused_sgd.fused_with_prox = True    # its step() leaves Ws to the call below
     for opt in self.optimizers:
       opt.step()
-    if fuse:
-      eng.sgd_prox_step(self._fused_sgd._lr(), prox_step_size, do_prox=True)
-    elif self.lam > 0:
+    if self._fused_sgd is not None:
+      self._fused_sgd.fused_with_prox = fuse
+      self.engine.sgd_prox_step(self._fused_sgd._lr(), prox_step_size if fuse else 0.0, do_prox=fuse,
+                                verdict=None if self._adamw is None else self._adamw._verdict())
+    elif fuse:
       self.generative_model.proximal_step(prox_step_size)
-    return self._info(out, scalars)
 
   def _small_step(self, X, eps, c, sig_off, pm, ps, prox_step_size):
     """The scripts' own small models (bars, mocap) on one GPU: the whole step is ONE launch (csrc/small_step.hip) --
@@ -151,15 +161,7 @@ class OIVAE(object):
       return self._info(out, out["scalars"].clone())
     out = eng.small_step(Xd, eps, c, prox_step_size, lr=0.0, Ws_lr=0.0, optimizers=False, **common)
     scalars = out["scalars"].clone()
-    fuse = self._fused_sgd is not None and self.lam > 0
-    if self._fused_sgd is not None:
-      self._fused_sgd.fused_with_prox = fuse
-    for opt in self.optimizers:
-      opt.step()
-    if fuse:
-      eng.sgd_prox_step(self._fused_sgd._lr(), prox_step_size, do_prox=True)
-    elif self.lam > 0:
-      self.generative_model.proximal_step(prox_step_size)
+    self._update(prox_step_size)
     return self._info(out, scalars)
 
   def evaluate(self, X, mc_samples, eps=None):

@@ -244,6 +244,8 @@ class AdamW(_EngineOptimizer):
 
   max_grad_norm: clips by the norm of all gradients of this optimizer (`grad_norm` holds it after a step).  The gradients
   themselves stay as they are, and a step whose norm is not finite is left out on the device (`skipped` counts them).
+  Handed to OIVAE, the norm is that of every gradient but Ws's, which SGD applies unclipped; a gradient of Ws that is not
+  finite leaves the step out too (the norm is NaN then), and a step that is left out leaves Ws alone as well.
   capturable: keeps the step counts on the device, so that a step captured into a graph advances them (max_grad_norm
   implies it); `lr` may then be a one-element float32 tensor on the device, which replays read anew.  Touch `buffers` (or
   take a step) before capturing.  Nothing here synchronises."""
@@ -339,9 +341,14 @@ class AdamW(_EngineOptimizer):
     self._groups_at = self._groups.ctypes.data
     self._clip = torch.zeros(8, dtype=torch.int32, device=device) if self._on_device else None
     if self._on_device:
-      self._ws = torch.empty(self._lib.oivae_grad_norm_workspace_bytes(len(leaves)), dtype=torch.uint8, device=device)
-      self._norm_rec = np.zeros(len(leaves), _GRAD)   # the gradients of all kinds, one behind the other
+      # the gradients of all kinds, one behind the other; on an engine then that of Ws, which is not clipped but leaves the
+      # step out as well when it is not finite
+      watched = [] if self._engine is None else [self._engine.g["Ws"]]
+      self._norm_rec = np.zeros(len(leaves) + len(watched), _GRAD)
+      for r, g in zip(self._norm_rec[len(leaves):], watched):
+        r["g"], r["n"], r["type"], r["index"] = g.data_ptr(), g.numel(), _lib.F32_WATCHED, -1
       self._norm_at = self._norm_rec.ctypes.data
+      self._ws = torch.empty(self._lib.oivae_grad_norm_workspace_bytes(len(self._norm_rec)), dtype=torch.uint8, device=device)
       at = 0
       for k in self._kinds:
         k.grads = self._norm_rec[at:at + len(k.mine)]
@@ -380,6 +387,10 @@ class AdamW(_EngineOptimizer):
       raise RuntimeError("AdamW computes the gradient norm where max_grad_norm is given")
     self.buffers
     return self._clip.view(torch.float32)[0]
+
+  def _verdict(self):
+    """Address of the last step's verdict (oivae_clip_t), None where none is formed."""
+    return self._clip.data_ptr() if self._on_device else None
 
   @property
   def skipped(self):
