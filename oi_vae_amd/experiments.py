@@ -27,8 +27,13 @@ class Experiment(object):
                lr=1e-3, Ws_lr=1e-4, lam=1.0, lam_adjustment=1.0, prior_theta_scale=1.0,
                prior_rows=1, native_optimizers=True, device=None, device_eps=False,
                weight_decay=None, state_bits=32, max_grad_norm=None):
-    """weight_decay (a number): the engine's AdamW instead of Adam, with its state_bits and max_grad_norm."""
+    """weight_decay (a number, 0 for none): the engine's AdamW instead of Adam, with its state_bits and max_grad_norm.  These
+    options are refused where AdamW is not chosen."""
     assert sum(group_dims) == dim_x
+    if weight_decay is None and (state_bits != 32 or max_grad_norm is not None):
+      raise ValueError("state_bits and max_grad_norm are AdamW's: give weight_decay too (0 for none)")
+    if weight_decay is not None and not native_optimizers:
+      raise ValueError("weight_decay, state_bits and max_grad_norm are the native AdamW's: not with native_optimizers=False")
     self.stddev_multiple = 0.1  # bars_data_oivae.py:60; read through the closure below on every step
     self.lam, self.lam_adjustment, self.Ws_lr = lam, lam_adjustment, Ws_lr
     self.inference_net = NormalNet(

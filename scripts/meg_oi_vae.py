@@ -52,6 +52,8 @@ def main(argv=None):
   ap.add_argument("--max-grad-norm", type=float, default=None, help="clip AdamW's gradients by their norm")
   ap.add_argument("--out", default="out_meg")
   args = ap.parse_args(argv)
+  if args.weight_decay is None and (args.state_bits != 32 or args.max_grad_norm is not None):
+    ap.error("--state-bits and --max-grad-norm are AdamW's: give --weight-decay too (0 for none)")
 
   world = int(os.environ.get("WORLD_SIZE", "1"))
   rank = int(os.environ.get("RANK", "0"))

@@ -34,3 +34,29 @@ def test_sgd_prox_clip_refuses_what_sgd_prox_does():
     rc = L.oivae_sgd_prox_f32(*args, 0.1, 1.0, 1, None, None, None)
     assert rc in (1, 2) and L.oivae_sgd_prox_clip_f32(*args, 0.1, 1.0, 1, None, None, None, None) == rc
     assert b"oivae_sgd_prox_clip_f32" in L.oivae_last_error()
+
+
+def _script(name):
+  import importlib.util
+  import os
+  path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "scripts", name + ".py")
+  spec = importlib.util.spec_from_file_location(name, path)
+  mod = importlib.util.module_from_spec(spec)
+  spec.loader.exec_module(mod)
+  return mod
+
+
+@pytest.mark.parametrize("kw", [dict(max_grad_norm=1.0), dict(state_bits=8), dict(weight_decay=0.01, native_optimizers=False),
+                                dict(weight_decay=0.01, max_grad_norm=1.0, native_optimizers=False),
+                                dict(max_grad_norm=1.0, native_optimizers=False)])
+def test_an_experiment_refuses_options_it_would_drop(kw):
+  from oi_vae_amd.experiments import Experiment
+  with pytest.raises(ValueError, match="AdamW's"):
+    Experiment(dim_x=8, dim_z=4, group_dims=[4, 4], group_input_dim=2, **kw)
+
+
+@pytest.mark.parametrize("argv", [["--max-grad-norm", "1"], ["--state-bits", "8"], ["--state-bits", "8", "--max-grad-norm", "1"]])
+def test_the_meg_driver_refuses_options_it_would_drop(argv, capsys):
+  with pytest.raises(SystemExit) as e:
+    _script("meg_oi_vae").main(argv)
+  assert e.value.code == 2 and "--weight-decay" in capsys.readouterr().err
