@@ -63,6 +63,8 @@ def main(argv=None):
   ap.add_argument("--max-grad-norm", type=float, default=None, help="adamw: clip the gradients by their norm")
   ap.add_argument("--out", default="out_autoencoder/data_vs_test_loss.json")
   args = ap.parse_args(argv)
+  if args.optimizer != "adamw" and (args.weight_decay != 0.0 or args.state_bits != 32 or args.max_grad_norm is not None):
+    ap.error("--weight-decay, --state-bits and --max-grad-norm are AdamW's: give --optimizer adamw too")
   if not torch.cuda.is_available():
     raise SystemExit("this script trains on the GPU (the proximal step has no CPU path)")
   dev = torch.device("cuda", 0)

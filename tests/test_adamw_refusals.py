@@ -60,3 +60,10 @@ def test_the_meg_driver_refuses_options_it_would_drop(argv, capsys):
   with pytest.raises(SystemExit) as e:
     _script("meg_oi_vae").main(argv)
   assert e.value.code == 2 and "--weight-decay" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("argv", [["--max-grad-norm", "1"], ["--state-bits", "8"], ["--weight-decay", "0.1"], ["--optimizer", "adam", "--weight-decay", "0.1"]])
+def test_the_autoencoder_driver_refuses_options_it_would_drop(argv, capsys):
+  with pytest.raises(SystemExit) as e:
+    _script("data_vs_test_loss_autoencoder").main(argv)
+  assert e.value.code == 2 and "--optimizer adamw" in capsys.readouterr().err
