@@ -308,7 +308,7 @@ typedef struct {
   int32_t group;     /* index into the groups */
   int32_t index;     /* of its step counter; distinguishes its random bits (oivae_adamw_f8) */
   int32_t step;      /* t >= 1, the step being taken; not read where the state holds step counters */
-  int32_t pad;
+  int32_t pad;       /* the caller's, not read */
 } oivae_adamw_tensor_t;
 
 typedef struct {

@@ -31,6 +31,19 @@ bool plain(const at::Tensor& t, int device) {
          (t.is_contiguous() || t.is_non_overlapping_and_dense());
 }
 
+// The order of a dense tensor's elements in memory: 0 row by row, else a number that another order hardly shares (a hash of
+// the sizes and strides of the dimensions that have any).  Moments lie in the order their parameter had at first.
+int32_t order_of(const at::Tensor& t) {
+  if (t.is_contiguous()) return 0;
+  uint32_t h = 2166136261u;
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) == 1) continue;
+    h = (h ^ (uint32_t)t.size(d)) * 16777619u;
+    h = (h ^ (uint32_t)t.stride(d)) * 16777619u;
+  }
+  return (int32_t)(h | 1u);
+}
+
 // what autograd is told where a kernel writes a tensor behind its back: a graph that saved it says so instead of going on
 void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -53,7 +66,7 @@ struct Buffer {
 
 // parameters(list, records of oivae_adamw_tensor_t, device, records of oivae_grad_t or None) -> (first unusual tensor or -1,
 // number without a gradient).  Fills p, g and g_type, g = 0 where a parameter has no gradient, and the gradients' records
-// (n = 0 and index -1 there).  The records' n and p_type say what the parameters have to be.
+// (n = 0 and index -1 there).  The records' n, p_type and pad (the order of its elements) say what the parameters have to be.
 PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 4 || !PyList_Check(args[0])) {
     PyErr_SetString(PyExc_TypeError, "parameters(list, records, device, gradient records)");
@@ -86,6 +99,7 @@ PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (!plain(p, (int)device) || !plain(g, (int)device) || p.numel() != r[i].n || type_of(p) != r[i].p_type || !g.sizes().equals(p.sizes()))
         break;
       if (!(p.is_contiguous() && g.is_contiguous()) && !g.strides().equals(p.strides())) break;
+      if (order_of(p) != r[i].pad) break;
       written(p);
       r[i].p = p.data_ptr();
       r[i].g = g.data_ptr();
@@ -141,7 +155,22 @@ PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return Py_BuildValue("(liK)", count, device, (unsigned long long)reinterpret_cast<uintptr_t>(r));
 }
 
+// order(tensor) -> order_of
+PyObject* order(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 1 || !THPVariable_Check(args[0])) {
+    PyErr_SetString(PyExc_TypeError, "order(tensor)");
+    return nullptr;
+  }
+  try {
+    return PyLong_FromLong(order_of(THPVariable_Unpack(args[0])));
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 PyMethodDef methods[] = {
+    {"order", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(order)), METH_FASTCALL, nullptr},
     {"parameters", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(parameters)), METH_FASTCALL, nullptr},
     {"gradients", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gradients)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -105,7 +105,7 @@ class SGD(_EngineOptimizer):
 _TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _GRAD = np.dtype([("g", "u8"), ("n", "i8"), ("type", "i4"), ("index", "i4")])                     # oivae_grad_t
 _TENSOR = np.dtype([("p", "u8"), ("g", "u8"), ("n", "i8"), ("at", "i8"), ("p_type", "i4"), ("g_type", "i4"),
-                    ("group", "i4"), ("index", "i4"), ("step", "i4"), ("pad", "i4")])             # oivae_adamw_tensor_t
+                    ("group", "i4"), ("index", "i4"), ("step", "i4"), ("order", "i4")])           # oivae_adamw_tensor_t
 _GROUP = np.dtype([("lr", "f4"), ("weight_decay", "f4"), ("lr_dev", "u8")])                       # oivae_adamw_group_t
 
 
@@ -377,8 +377,21 @@ class AdamW(_EngineOptimizer):
   def sync_master(self):
     """Takes the master weights of 16-bit parameters from the parameters again."""
     self.buffers
+    for k in self._kinds:
+      for p, r in zip(k.leaves, k.rec):
+        self._check_parameter(p, r)
     for p, flat in self._views("master"):
       flat.as_strided(p.shape, p.stride()).copy_(p)
+
+  def _check_parameter(self, p, r):
+    """Refuses a parameter that is not what its moments were made for."""
+    if p.numel() != r["n"] or _TYPES.get(p.dtype) != r["p_type"]:
+      raise ValueError("a parameter changed its size or type since this optimizer's first step")
+    if not _dense(p):
+      raise ValueError("a parameter of strides %s and shape %s does not fill its memory" % (p.stride(), tuple(p.shape)))
+    if _lists().order(p) != r["order"]:
+      raise ValueError("a parameter changed the order of its elements since this optimizer's first step: its moments lie in that "
+                       "one, now it has strides %s" % (p.stride(),))
 
   @property
   def grad_norm(self):
@@ -473,12 +486,9 @@ class AdamW(_EngineOptimizer):
       if g.dtype not in _TYPES or g.device != self.device or p.device != self.device:
         raise ValueError("parameter and gradient must be float32, bfloat16 or float16 on %s, got %s on %s with %s on %s"
                          % (self.device, p.dtype, p.device, g.dtype, g.device))
-      if p.numel() != r["n"] or _TYPES.get(p.dtype) != r["p_type"]:
-        raise ValueError("a parameter changed its size or type since this optimizer's first step")
+      self._check_parameter(p, r)
       if g.shape != p.shape:
         raise ValueError("a gradient of shape %s for a parameter of shape %s" % (tuple(g.shape), tuple(p.shape)))
-      if not _dense(p):
-        raise ValueError("a parameter of strides %s and shape %s does not fill its memory" % (p.stride(), tuple(p.shape)))
       if g.is_neg() or (g.stride() != p.stride() and not (p.is_contiguous() and g.is_contiguous())):
         g = torch.empty_like(p, dtype=g.dtype).copy_(g)
         copies.append(g)
@@ -576,6 +586,7 @@ class _Kind(object):
     rec["p_type"] = [_TYPES[p.dtype] for p in self.leaves]
     rec["group"] = [groups[i] for i in mine]
     rec["index"] = mine
+    rec["order"] = [_lists().order(p) for p in self.leaves]
     self.rec_at = rec.ctypes.data
     total, half = max(int(whole.sum()), _lib.ADAMW_BLOCK), int(whole[rec["p_type"] != _lib.F32].sum())
     self.held = held = {}

@@ -67,3 +67,16 @@ def test_the_autoencoder_driver_refuses_options_it_would_drop(argv, capsys):
   with pytest.raises(SystemExit) as e:
     _script("data_vs_test_loss_autoencoder").main(argv)
   assert e.value.code == 2 and "--optimizer adamw" in capsys.readouterr().err
+
+
+def test_order_of_elements():
+  """Row by row is 0, whatever the strides of dimensions of one element; other orders differ from it and from each other."""
+  from oi_vae_amd import _tensor_lists
+  order, x = _tensor_lists.order, torch.zeros(4, 6, 5)
+  assert order(x) == 0 == order(x.view(24, 5)) == order(x.new_zeros(0, 3)) == order(x.new_zeros(())) == order(x.new_zeros(7, 1).t())
+  others = [x.permute(2, 0, 1), x.permute(2, 1, 0), x.permute(1, 0, 2), x.new_zeros(24, 5).t(), x.new_zeros(5, 24).t()]
+  codes = [order(t) for t in others]
+  assert 0 not in codes and len(set(codes)) == len(codes)
+  assert codes == [order(torch.empty_like(t)) for t in others] == [order(t[None]) for t in others]
+  with pytest.raises(TypeError):
+    order(3)
