@@ -326,7 +326,7 @@ class AdamW(_EngineOptimizer):
     spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in leaves if p.numel())
     if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
       raise ValueError("two parameters share memory")
-    self._leaves, self.device = leaves, device
+    self._leaves, self._group_of, self.device = leaves, groups, device
     self._lib = _lib.init_device(device.index)
     self._kinds = []
     self._steps_dev = torch.zeros(len(leaves), 4, dtype=torch.int32, device=device) if self._on_device else None
@@ -437,13 +437,21 @@ class AdamW(_EngineOptimizer):
   def state_dict(self):
     """Everything a resumed run needs: counts, options and copies of `buffers`."""
     self.buffers
-    return {"steps": self.steps(), "seed": self.seed, "sizes": [p.numel() for p in self._leaves],
+    return {"steps": self.steps(), "seed": self.seed, "sizes": [p.numel() for p in self._leaves], **self._layout(),
             "groups": [{k: v.clone() if torch.is_tensor(v) else v for k, v in g.items() if k != "params"} for g in self.param_groups],
             "buffers": {bits: {k: t.clone() for k, t in held.items()} for bits, held in self.buffers.items()}}
 
+  def _layout(self):
+    """What decides, beside the sizes, where in the buffers a parameter's state lies and which options it has."""
+    types, orders = [None] * len(self._leaves), [None] * len(self._leaves)
+    for k in self._kinds:
+      for i, r in zip(k.mine, k.rec):
+        types[i], orders[i] = ("float32", "bfloat16", "float16")[r["p_type"]], int(r["order"])
+    return {"types": types, "orders": orders, "group_of": list(self._group_of)}
+
   @torch.no_grad()
   def load_state_dict(self, state):
-    """Takes over a state_dict of an AdamW over parameters of the same sizes, types and groups; all or nothing."""
+    """Takes over a state_dict of an AdamW over parameters of the same sizes, types, orders in memory and groups."""
     held = self.buffers
     for what, mine, theirs in [("bits", held, state["buffers"])] + [("buffers", held[b], state["buffers"].get(b, {})) for b in held]:
       if sorted(mine) != sorted(theirs):
@@ -455,6 +463,15 @@ class AdamW(_EngineOptimizer):
     if (list(state["sizes"]) != [p.numel() for p in self._leaves] or len(state["groups"]) != len(self.param_groups)
         or any(src["state_bits"] != g["state_bits"] for src, g in zip(state["groups"], self.param_groups))):
       raise ValueError("the state was made for other parameters or groups")
+    layout = self._layout()
+    if any(k in state for k in layout):
+      for k, mine in layout.items():
+        if list(state.get(k, ())) != mine:
+          raise ValueError("the state was made for other parameters or groups: %s %s there, %s here" % (k, state.get(k), mine))
+    elif len(self._kinds) != 1 or len({t == "float32" for t in layout["types"]}) != 1:
+      # written before states held their layout: the sizes alone say where everything lies where the moments have one number of
+      # bits and the parameters are all of 32 or all of 16
+      raise ValueError("the state was made for parameters of unknown types and groups, which these do not tell")
     for t, src, _ in pairs:
       t.view(torch.uint8).copy_(src.view(torch.uint8))
     self.set_steps(state["steps"])

@@ -38,3 +38,62 @@ def test_a_parameter_that_changes_the_order_of_its_elements_is_refused(typ, clip
     p.data = torch.empty_like(x).copy_(p.data)
     opt.step()
     assert opt.steps() == [3] and not torch.equal(was[0], p)
+
+
+def _made(kinds, **kw):
+  """An AdamW over groups of parameters given as [(type, size, row-major?), ...], one step taken."""
+  from oi_vae_amd import optim
+  g = torch.Generator(device="cuda").manual_seed(len(kinds))
+  groups = []
+  for k, members in enumerate(kinds):
+    ps = []
+    for typ, shape, rows in members:
+      x = torch.randn(shape, generator=g, device="cuda").to(TYPES[typ])
+      p = (x if rows else x.t().contiguous().t()).requires_grad_()
+      p.grad = torch.ones_like(p)
+      ps.append(p)
+    groups.append({"params": ps, "weight_decay": 0.01 * k})
+  opt = optim.AdamW(groups, lr=1e-2, **kw)
+  opt.step()
+  return opt, [p for q in groups for p in q["params"]]
+
+
+A, B = ("f32", (128,), True), ("bf16", (128,), True)
+M, T = ("f32", (8, 16), True), ("f32", (8, 16), False)
+
+
+@pytest.mark.parametrize("clip", [None, 1.0])
+@pytest.mark.parametrize("theirs,mine", [([[A, B]], [[B, A]]),                 # equal sizes, types changed places
+                                         ([[B, B]], [[("f16", (128,), True), B]]),
+                                         ([[M, M]], [[M, T]]),                 # another order in memory
+                                         ([[A, A], [A]], [[A], [A, A]]),       # another group
+                                         ([[A, B], [B]], [[A], [B, B]])])
+def test_a_state_of_other_types_orders_or_groups_is_refused(theirs, mine, clip):
+  state = _made(theirs, max_grad_norm=clip)[0].state_dict()
+  opt, ps = _made(mine, max_grad_norm=clip)
+  was, steps = _snapshot(opt, ps), opt.steps()
+  with pytest.raises(ValueError, match="other parameters or groups"):
+    opt.load_state_dict(state)
+  assert steps == opt.steps() and all(torch.equal(a, b) for a, b in zip(was, _snapshot(opt, ps)))
+  opt, ps = _made(theirs, max_grad_norm=clip)
+  opt.step()
+  opt.load_state_dict(state)
+  assert opt.steps() == steps
+
+
+def test_states_from_before_they_held_their_layout():
+  """Taken where the sizes decide the layout, refused where they do not."""
+  for kinds, taken in (([[A, M]], True), ([[B, B]], True), ([[A, B]], False), ([[A], [A]], True)):
+    opt, ps = _made(kinds)
+    state = opt.state_dict()
+    for k in ("types", "orders", "group_of"):
+      del state[k]
+    opt.step()
+    was = _snapshot(opt, ps)
+    if taken:
+      opt.load_state_dict(state)
+      assert opt.steps() == [1] * len(ps)
+    else:
+      with pytest.raises(ValueError, match="unknown types"):
+        opt.load_state_dict(state)
+      assert all(torch.equal(a, b) for a, b in zip(was, _snapshot(opt, ps)))
