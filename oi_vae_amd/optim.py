@@ -37,9 +37,9 @@ class _EngineOptimizer(object):
       self.param_groups.append(d)
     self._engine = None
 
-  def _uniform(self, key):
+  def _uniform(self, key, groups=None):
     """The one value of an option across all param groups (read at step time: schedulers may change it)."""
-    vals = {(tuple(g[key]) if isinstance(g[key], (list, tuple)) else g[key]) for g in self.param_groups}
+    vals = {(tuple(g[key]) if isinstance(g[key], (list, tuple)) else g[key]) for g in groups or self.param_groups}
     if len(vals) != 1:
       raise ValueError("engine-native optimizers apply one %r to every param group, got %s" % (key, sorted(vals)))
     return vals.pop()
@@ -255,8 +255,7 @@ class AdamW(_EngineOptimizer):
     super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits)
     if max_grad_norm is not None and not max_grad_norm > 0:
       raise ValueError("max_grad_norm must be positive or None, got %r" % (max_grad_norm,))
-    if not 0 <= int(seed) < 1 << 32:
-      raise ValueError("seed must be in [0, 2^32), got %r" % (seed,))
+    seed = self._checked_seed(seed)
     seen = set()
     for g in self.param_groups:
       if g["state_bits"] not in (8, 32):
@@ -269,18 +268,25 @@ class AdamW(_EngineOptimizer):
       raise ValueError("AdamW got no parameters")
     self._options()
     self.max_grad_norm = max_grad_norm
-    self.seed = int(seed)
+    self.seed = seed
     self._on_device = bool(capturable) or max_grad_norm is not None
     self._buffers = None
 
-  def _options(self):
-    b1, b2 = self._uniform("betas")
-    eps = self._uniform("eps")
+  @staticmethod
+  def _checked_seed(seed):
+    if not 0 <= int(seed) < 1 << 32:
+      raise ValueError("seed must be in [0, 2^32), got %r" % (seed,))
+    return int(seed)
+
+  def _options(self, groups=None):
+    groups = groups or self.param_groups
+    b1, b2 = self._uniform("betas", groups)
+    eps = self._uniform("eps", groups)
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
       raise ValueError("betas must be in [0, 1), got %r" % ((b1, b2),))
     if not eps >= 0.0:
       raise ValueError("eps must not be negative, got %r" % (eps,))
-    for g in self.param_groups:
+    for g in groups:
       if not torch.is_tensor(g["lr"]) and not g["lr"] >= 0.0:
         raise ValueError("lr must not be negative, got %r" % (g["lr"],))
       if not g["weight_decay"] >= 0.0:
@@ -423,12 +429,16 @@ class AdamW(_EngineOptimizer):
       counts[k.mine] = k.rec["step"]
     return counts.tolist()
 
-  def set_steps(self, steps):
-    """Sets the step counts: one number for all parameters or one for each."""
-    self.buffers
+  def _counts(self, steps):
     counts = np.broadcast_to(np.asarray(steps, np.int32), (len(self._leaves),))
     if (counts < 0).any():
       raise ValueError("step counts must not be negative")
+    return counts
+
+  def set_steps(self, steps):
+    """Sets the step counts: one number for all parameters or one for each."""
+    self.buffers
+    counts = self._counts(steps)
     for k in self._kinds:
       k.rec["step"] = counts[k.mine]
     if self._on_device:
@@ -451,8 +461,12 @@ class AdamW(_EngineOptimizer):
 
   @torch.no_grad()
   def load_state_dict(self, state):
-    """Takes over a state_dict of an AdamW over parameters of the same sizes, types, orders in memory and groups."""
+    """Takes over a state_dict of an AdamW over parameters of the same sizes, types, orders in memory and groups; any other is
+    refused before anything is changed."""
     held = self.buffers
+    lacking = [k for k in ("steps", "seed", "sizes", "groups", "buffers") if k not in state]
+    if lacking:
+      raise ValueError("the state holds no %s" % ", ".join(lacking))
     for what, mine, theirs in [("bits", held, state["buffers"])] + [("buffers", held[b], state["buffers"].get(b, {})) for b in held]:
       if sorted(mine) != sorted(theirs):
         raise ValueError("the state holds %s %s, this optimizer %s" % (what, sorted(theirs), sorted(mine)))
@@ -472,16 +486,35 @@ class AdamW(_EngineOptimizer):
       # written before states held their layout: the sizes alone say where everything lies where the moments have one number of
       # bits and the parameters are all of 32 or all of 16
       raise ValueError("the state was made for parameters of unknown types and groups, which these do not tell")
+    if len(state["steps"]) != len(self._leaves):
+      raise ValueError("the state holds %d step counts for %d parameters" % (len(state["steps"]), len(self._leaves)))
+    counts, seed, options = self._counts(state["steps"]), self._checked_seed(state["seed"]), self._options_from(state["groups"])
     for t, src, _ in pairs:
       t.view(torch.uint8).copy_(src.view(torch.uint8))
-    self.set_steps(state["steps"])
-    self.seed = state["seed"]
-    for g, src in zip(self.param_groups, state["groups"]):
+    self.set_steps(counts)
+    self.seed = seed
+    for g, src in zip(self.param_groups, options):
       for k, v in src.items():
         if torch.is_tensor(g[k]):
-          g[k].copy_(torch.as_tensor(v))     # an lr on the device stays where a captured graph reads it
+          g[k].fill_(v)     # an lr on the device stays where a captured graph reads it
         else:
-          g[k] = v.item() if torch.is_tensor(v) else v
+          g[k] = v
+
+  def _options_from(self, groups):
+    """A state's options, as numbers, once they are known to be ones that this optimizer's groups could have been given."""
+    out = []
+    for g, src in zip(self.param_groups, groups):
+      if set(src) != set(g) - {"params"}:
+        raise ValueError("a group of the state has the options %s, here it has %s" % (sorted(src), sorted(set(g) - {"params"})))
+      for k, v in list(src.items()) + [(k, v) for k, v in g.items() if k != "params"]:
+        if torch.is_tensor(v) and v.numel() != 1:
+          raise ValueError("%s has %d values" % (k, v.numel()))
+      out.append({k: v.item() if torch.is_tensor(v) else v for k, v in src.items()})
+    self._options(out)
+    if self._engine is not None:
+      for key in ("lr", "weight_decay"):
+        self._uniform(key, out)
+    return out
 
   # ---- the step ---------------------------------------------------------------
   @torch.no_grad()

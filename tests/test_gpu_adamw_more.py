@@ -97,3 +97,36 @@ def test_states_from_before_they_held_their_layout():
       with pytest.raises(ValueError, match="unknown types"):
         opt.load_state_dict(state)
       assert all(torch.equal(a, b) for a, b in zip(was, _snapshot(opt, ps)))
+
+
+@pytest.mark.parametrize("clip", [None, 1.0])
+@pytest.mark.parametrize("change", [lambda s: s["groups"][1].update(initial_lr=1e-2), lambda s: s["groups"][0].pop("eps"),
+                                    lambda s: s["groups"][0].update(lr=-1.0), lambda s: s["groups"][1].update(betas=(0.8, 0.9)),
+                                    lambda s: s["groups"][0].update(lr=torch.zeros(2)), lambda s: s["groups"][0].update(weight_decay=float("nan")),
+                                    lambda s: s["steps"].pop(), lambda s: s["steps"].append(1), lambda s: s.update(steps=[1, -1, 1]),
+                                    lambda s: s.update(steps=[1, 1 << 40, 1]), lambda s: s.update(seed=1 << 32), lambda s: s.pop("seed"),
+                                    lambda s: s.pop("steps"), lambda s: s.pop("buffers"), lambda s: s["buffers"][32].pop("exp_avg_sq")])
+def test_a_state_is_taken_whole_or_not_at_all(change, clip):
+  opt, ps = _made([[A, B], [B]], max_grad_norm=clip)
+  state = opt.state_dict()
+  change(state)
+  opt.step()
+  options = [{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups]
+  was, steps, seed = _snapshot(opt, ps), opt.steps(), opt.seed
+  with pytest.raises((ValueError, OverflowError)):
+    opt.load_state_dict(state)
+  assert steps == opt.steps() and seed == opt.seed and all(torch.equal(a, b) for a, b in zip(was, _snapshot(opt, ps)))
+  assert options == [{k: v for k, v in g.items() if k != "params"} for g in opt.param_groups]
+
+
+@pytest.mark.parametrize("there,here", [(1e-3, None), (None, 1e-3), (None, None), ("0-dim", None), (None, "0-dim")])
+def test_learning_rates_of_a_state(there, here):
+  """A number or one float32 on the device (of any shape of one element) on either side; the one here stays in place."""
+  def lr(what, value):
+    return value if what is not None and what != "0-dim" else torch.full(() if what else (1,), value, device="cuda")
+  opt, ps = _made([[A]], capturable=True)
+  opt.param_groups[0]["lr"] = lr(there, 0.25)
+  state = opt.state_dict()
+  mine = opt.param_groups[0]["lr"] = lr(here, 0.5)
+  opt.load_state_dict(state)
+  assert float(opt.param_groups[0]["lr"]) == 0.25 and (opt.param_groups[0]["lr"] is mine or not torch.is_tensor(mine))
