@@ -448,6 +448,7 @@ class AdamW(_EngineOptimizer):
     """Everything a resumed run needs: counts, options and copies of `buffers`."""
     self.buffers
     return {"steps": self.steps(), "seed": self.seed, "sizes": [p.numel() for p in self._leaves], **self._layout(),
+            "skipped": int(self._clip[3]) if self._on_device else 0,
             "groups": [{k: v.clone() if torch.is_tensor(v) else v for k, v in g.items() if k != "params"} for g in self.param_groups],
             "buffers": {bits: {k: t.clone() for k, t in held.items()} for bits, held in self.buffers.items()}}
 
@@ -488,11 +489,16 @@ class AdamW(_EngineOptimizer):
       raise ValueError("the state was made for parameters of unknown types and groups, which these do not tell")
     if len(state["steps"]) != len(self._leaves):
       raise ValueError("the state holds %d step counts for %d parameters" % (len(state["steps"]), len(self._leaves)))
+    skipped = int(state.get("skipped", 0))
+    if not 0 <= skipped < 1 << 31:
+      raise ValueError("the state counts %r steps left out" % (skipped,))
     counts, seed, options = self._counts(state["steps"]), self._checked_seed(state["seed"]), self._options_from(state["groups"])
     for t, src, _ in pairs:
       t.view(torch.uint8).copy_(src.view(torch.uint8))
     self.set_steps(counts)
     self.seed = seed
+    if self._on_device:
+      self._clip[3] = skipped
     for g, src in zip(self.param_groups, options):
       for k, v in src.items():
         if torch.is_tensor(g[k]):

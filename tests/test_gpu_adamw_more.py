@@ -130,3 +130,27 @@ def test_learning_rates_of_a_state(there, here):
   mine = opt.param_groups[0]["lr"] = lr(here, 0.5)
   opt.load_state_dict(state)
   assert float(opt.param_groups[0]["lr"]) == 0.25 and (opt.param_groups[0]["lr"] is mine or not torch.is_tensor(mine))
+
+
+def test_steps_left_out_are_counted_on_after_resuming():
+  opt, ps = _made([[A, B]], max_grad_norm=1.0)
+  ps[0].grad[3] = float("nan")
+  for _ in range(2):
+    opt.step()
+  state = opt.state_dict()
+  assert state["skipped"] == 2 and state["steps"] == [1, 1]
+  other, qs = _made([[A, B]], max_grad_norm=1.0)
+  other.load_state_dict(state)
+  assert other.skipped.item() == 2
+  qs[1].grad[0] = float("inf")
+  other.step()
+  assert other.skipped.item() == 3 and other.steps() == [1, 1]
+  for bad in (-1, 1 << 31):
+    with pytest.raises(ValueError, match="left out"):
+      other.load_state_dict({**state, "skipped": bad})
+  del state["skipped"]          # a state from before they were held
+  other.load_state_dict(state)
+  assert other.skipped.item() == 0
+  plain = _made([[A, B]])[0]
+  assert plain.state_dict()["skipped"] == 0
+  plain.load_state_dict({**state, "skipped": 5})
