@@ -193,7 +193,7 @@ def _clip(got, max_norm):
   L = _lib.init_device(device)
   nbytes = L.oivae_grad_norm_workspace_bytes(count)
   # norm and workspace of this call alone: calls on other streams and in captured graphs have their own
-  norm, ws = torch.empty((), device="cuda"), torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+  norm, ws = torch.empty((), dtype=torch.float32, device="cuda"), torch.empty(nbytes, dtype=torch.uint8, device="cuda")
   _lib.check(L.oivae_clip_grad_norm(address, count, max_norm, norm.data_ptr(), ws.data_ptr(), nbytes,
                                     _stream(device)), "oivae_clip_grad_norm")
   return norm
@@ -201,11 +201,11 @@ def _clip(got, max_norm):
 
 def grad_norm(parameters):
   """2-norm of the gradients of `parameters` (a tensor or an iterable of tensors; those without a gradient are left out)
-  taken as one vector: a 0-dim float32 tensor on their device, with no synchronisation.  Squares and sums are formed in
+  taken as one vector: a 0-dim float32 tensor on their device (a zero on the CPU without any), with no synchronisation.  Squares and sums are formed in
   fp64, in an order that depends on the sizes alone."""
   got = _grads_of(parameters, False)
   if got is None:
-    return torch.zeros(())
+    return torch.zeros((), dtype=torch.float32)
   return _clip(got, 0.0)
 
 
@@ -217,7 +217,7 @@ def clip_grad_norm_(parameters, max_norm):
     raise ValueError("max_norm must be positive, got %r" % max_norm)
   got = _grads_of(parameters, True)
   if got is None:
-    return torch.zeros(())
+    return torch.zeros((), dtype=torch.float32)
   norm = _clip(got, max_norm)
   if got[4]:
     with torch.no_grad():

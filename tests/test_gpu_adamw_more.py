@@ -154,3 +154,23 @@ def test_steps_left_out_are_counted_on_after_resuming():
   plain = _made([[A, B]])[0]
   assert plain.state_dict()["skipped"] == 0
   plain.load_state_dict({**state, "skipped": 5})
+
+
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
+def test_under_another_default_type(default):
+  """torch.set_default_dtype changes nothing: the norm is a float32, the step the same."""
+  from oi_vae_amd import optim
+
+  def run(default):
+    ps = _params([300, 5000], torch.float32, seed=3)
+    torch.set_default_dtype(default)
+    try:
+      opt = optim.AdamW(ps, lr=1e-2, max_grad_norm=0.1)
+      opt.step()
+      norms = [optim.grad_norm(ps), opt.grad_norm, optim.clip_grad_norm_(ps, 0.1), optim.grad_norm([]), optim.clip_grad_norm_([], 1.0)]
+    finally:
+      torch.set_default_dtype(torch.float32)
+    assert all(n.dtype == torch.float32 for n in norms)
+    return [n.item() for n in norms], _snapshot(opt, ps) + [p.grad.clone() for p in ps]
+  want, got = run(torch.float32), run(default)
+  assert got[0] == want[0] and all(torch.equal(a, b) for a, b in zip(got[1], want[1]))
