@@ -136,6 +136,14 @@ def _check_types(tensors, what):
   return device
 
 
+def _limit(max_norm, what="max_norm"):
+  """max_norm as a number, refused where float32, which the kernels compare in, has no positive value for it."""
+  number = float(max_norm)
+  if not number > 2.0 ** -150:     # half of float32's smallest
+    raise ValueError("%s must be positive (and not below float32's range), got %r" % (what, max_norm))
+  return number
+
+
 def _lists():
   """The native reader of tensor lists (csrc/tensor_lists.cpp)."""
   global _lists_module
@@ -212,9 +220,7 @@ def grad_norm(parameters):
 def clip_grad_norm_(parameters, max_norm):
   """torch.nn.utils.clip_grad_norm_ (2-norm): scales the gradients in place by min(1, max_norm / (norm + 1e-6)) and returns
   the norm they had, without synchronising.  A norm that is not finite reaches the gradients as it does there (NaN)."""
-  max_norm = float(max_norm)
-  if not max_norm > 0:
-    raise ValueError("max_norm must be positive, got %r" % max_norm)
+  max_norm = _limit(max_norm)
   got = _grads_of(parameters, True)
   if got is None:
     return torch.zeros((), dtype=torch.float32)
@@ -253,8 +259,8 @@ class AdamW(_EngineOptimizer):
   def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None,
                capturable=False, seed=0):
     super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits)
-    if max_grad_norm is not None and not max_grad_norm > 0:
-      raise ValueError("max_grad_norm must be positive or None, got %r" % (max_grad_norm,))
+    if max_grad_norm is not None:
+      _limit(max_grad_norm, "max_grad_norm")
     seed = self._checked_seed(seed)
     seen = set()
     for g in self.param_groups:

@@ -80,3 +80,16 @@ def test_order_of_elements():
   assert codes == [order(torch.empty_like(t)) for t in others] == [order(t[None]) for t in others]
   with pytest.raises(TypeError):
     order(3)
+
+
+@pytest.mark.parametrize("limit", [1e-50, 1e-46, 0.0, -1.0, float("nan"), -float("inf")])
+def test_limits_that_float32_does_not_hold_are_refused(limit):
+  """The kernels take the limit as a float32, where 0 means no clipping."""
+  from oi_vae_amd import optim
+  p = torch.zeros(3, requires_grad=True)
+  with pytest.raises(ValueError, match="max_norm must be positive"):
+    optim.clip_grad_norm_([p], limit)
+  with pytest.raises(ValueError, match="max_grad_norm must be positive"):
+    optim.AdamW([p], max_grad_norm=limit)
+  for fine in (1e-44, 1, np.float32(0.5), torch.tensor(2.0), 1e300, float("inf")):
+    optim.AdamW([p], max_grad_norm=fine)
