@@ -575,6 +575,8 @@ class AdamW(_EngineOptimizer):
     first, L, index = self.param_groups[0], self._lib, self.device.index
     (b1, b2), eps = first["betas"], first["eps"]
     groups = self._groups
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0):
+      self._options()      # says which; before the norm's launch, which advances the counts on the device
     for q, g in enumerate(self.param_groups):
       if g is not first and (g["eps"] != eps or tuple(g["betas"]) != (b1, b2)):
         raise ValueError("AdamW applies one 'betas' and one 'eps' to every param group")

@@ -174,3 +174,21 @@ def test_under_another_default_type(default):
     return [n.item() for n in norms], _snapshot(opt, ps) + [p.grad.clone() for p in ps]
   want, got = run(torch.float32), run(default)
   assert got[0] == want[0] and all(torch.equal(a, b) for a, b in zip(got[1], want[1]))
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(capturable=True), dict(max_grad_norm=1.0)])
+def test_options_that_became_bad_are_refused_before_anything_is_queued(kw):
+  """The counts on the device advance with the norm, ahead of the step: a refused step must not have moved them."""
+  opt, ps = _made([[A, B], [B]], **kw)
+  was = _snapshot(opt, ps)
+  for key, bad in (("eps", -1e-8), ("eps", float("nan")), ("betas", (1.0, 0.999)), ("betas", (0.9, -0.5)), ("betas", (0.9, float("nan")))):
+    keep = [g[key] for g in opt.param_groups]
+    for g in opt.param_groups:
+      g[key] = bad
+    with pytest.raises(ValueError, match="eps must|betas must|one 'betas'|one 'eps'|to every param group"):
+      opt.step()
+    for g, k in zip(opt.param_groups, keep):
+      g[key] = k
+    assert opt.steps() == [1, 1, 1] and all(torch.equal(a, b) for a, b in zip(was, _snapshot(opt, ps)))
+  opt.step()
+  assert opt.steps() == [2, 2, 2]
