@@ -407,7 +407,8 @@ class AdamW(_EngineOptimizer):
 
   @property
   def grad_norm(self):
-    """Norm of the last step's gradients (after grad_scale): a 0-dim tensor on the device.  Needs max_grad_norm."""
+    """Norm of the last step's gradients (after grad_scale): a 0-dim tensor on the device, a view of the optimizer's buffer that
+    the next step overwrites (clone it to keep it).  Needs max_grad_norm."""
     if self.max_grad_norm is None:
       raise RuntimeError("AdamW computes the gradient norm where max_grad_norm is given")
     self.buffers
@@ -419,7 +420,8 @@ class AdamW(_EngineOptimizer):
 
   @property
   def skipped(self):
-    """Number of steps left out because their gradient norm was not finite: a 0-dim int32 tensor on the device."""
+    """Number of steps left out because their gradient norm was not finite: a 0-dim int32 tensor on the device, a view of the
+    optimizer's buffer."""
     if not self._on_device:
       raise RuntimeError("AdamW leaves steps out where max_grad_norm (or capturable) is given")
     self.buffers
@@ -582,8 +584,11 @@ class AdamW(_EngineOptimizer):
         raise ValueError("AdamW applies one 'betas' and one 'eps' to every param group")
       lr = g["lr"]
       groups[q] = self._lr_on_device(lr, g) if torch.is_tensor(lr) else (lr, g["weight_decay"], 0)
-    if self.max_grad_norm is not None and not self._on_device:
-      raise RuntimeError("max_grad_norm has to be given to the constructor (it may be changed or set to None later)")
+    limit = 0.0
+    if self.max_grad_norm is not None:
+      limit = _limit(self.max_grad_norm, "max_grad_norm")
+      if not self._on_device:
+        raise RuntimeError("max_grad_norm has to be given to the constructor (it may be changed or set to None later)")
     if not self._on_device and torch.cuda.is_current_stream_capturing():
       raise RuntimeError("a captured step would repeat its step count at every replay: use AdamW(capturable=True)")
     todo, partial, copies = [], False, []
@@ -608,9 +613,7 @@ class AdamW(_EngineOptimizer):
     clip = None
     if self._on_device:
       clip = self._clip.data_ptr()
-      norm = self.max_grad_norm
-      _lib.check(L.oivae_grad_norm(self._norm_at, len(self._norm_rec), norm is not None, grad_scale,
-                                   0.0 if norm is None else float(norm), clip, self._steps_dev.data_ptr(), b1, b2,
+      _lib.check(L.oivae_grad_norm(self._norm_at, len(self._norm_rec), limit > 0.0, grad_scale, limit, clip, self._steps_dev.data_ptr(), b1, b2,
                                    self._ws.data_ptr(), self._ws.numel(), stream), "oivae_grad_norm")
     for k, rec in todo:
       if not len(rec):

@@ -192,3 +192,25 @@ def test_options_that_became_bad_are_refused_before_anything_is_queued(kw):
     assert opt.steps() == [1, 1, 1] and all(torch.equal(a, b) for a, b in zip(was, _snapshot(opt, ps)))
   opt.step()
   assert opt.steps() == [2, 2, 2]
+
+
+def test_a_limit_changed_between_steps():
+  """A later limit is used, or refused as the constructor refuses it -- not taken for none; None takes no norm."""
+  opt, ps = _made([[A, B]], max_grad_norm=1.0)
+  was = _snapshot(opt, ps)
+  for bad in (0.0, -1.0, float("nan"), 1e-50):
+    opt.max_grad_norm = bad
+    with pytest.raises(ValueError, match="max_grad_norm must be positive"):
+      opt.step()
+  assert opt.steps() == [1, 1] and all(torch.equal(a, b) for a, b in zip(was, _snapshot(opt, ps)))
+  norms = []
+  for limit in (0.5, 1e9):
+    for p in ps:
+      p.grad.mul_(2.0)
+    opt.max_grad_norm = limit
+    opt.step()
+    norms.append(opt.grad_norm.clone())        # (grad_norm itself is the optimizer's buffer: the last step's)
+  assert norms[1].item() == 2 * norms[0].item() and opt.grad_norm.item() == norms[1].item()
+  opt.max_grad_norm = None
+  opt.step()
+  assert opt.steps() == [4, 4]
