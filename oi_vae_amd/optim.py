@@ -318,7 +318,10 @@ class AdamW(_EngineOptimizer):
         if set_to_none:
           p.grad = None
         elif p.grad is not None:
-          p.grad.detach_()
+          if p.grad.grad_fn is not None:
+            p.grad.detach_()
+          else:
+            p.grad.requires_grad_(False)     # (detach_ refuses views, such as parts of a flat buffer of gradients)
           p.grad.zero_()
 
   # ---- storage ---------------------------------------------------------------

@@ -93,3 +93,17 @@ def test_limits_that_float32_does_not_hold_are_refused(limit):
     optim.AdamW([p], max_grad_norm=limit)
   for fine in (1e-44, 1, np.float32(0.5), torch.tensor(2.0), 1e300, float("inf")):
     optim.AdamW([p], max_grad_norm=fine)
+
+
+def test_zero_grad_in_place():
+  """Gradients that are views of a flat buffer, that have a graph of their own, and plain ones."""
+  from oi_vae_amd import optim
+  flat = torch.ones(10)
+  p, q, r = (torch.ones(5, requires_grad=True) for _ in range(3))
+  p.grad = flat[2:7]
+  (q ** 3).sum().backward(create_graph=True)
+  r.grad = torch.ones(5)
+  opt = optim.AdamW([p, q, r])
+  opt.zero_grad(set_to_none=False)
+  assert flat.tolist() == [1.0] * 2 + [0.0] * 5 + [1.0] * 3 and p.grad.data_ptr() == flat[2:].data_ptr()
+  assert all((t.grad == 0).all() and not t.grad.requires_grad for t in (p, q, r))
