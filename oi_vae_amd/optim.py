@@ -21,6 +21,8 @@ from . import _lib
 
 class _EngineOptimizer(object):
   def __init__(self, params, **defaults):
+    if torch.is_tensor(params):
+      raise TypeError("params must be an iterable of tensors or of groups, got one tensor (give [tensor])")
     groups = list(params)
     if groups and not isinstance(groups[0], dict):
       groups = [{"params": groups}]
@@ -33,7 +35,8 @@ class _EngineOptimizer(object):
                          % (type(self).__name__, ", ".join(extra), ", ".join(sorted(defaults))))
       d = dict(defaults)
       d.update({k: v for k, v in g.items() if k != "params"})
-      d["params"] = list(g["params"])
+      members = g["params"]
+      d["params"] = [members] if torch.is_tensor(members) else list(members)   # (list() of a tensor are its rows)
       self.param_groups.append(d)
     self._engine = None
 
@@ -267,6 +270,10 @@ class AdamW(_EngineOptimizer):
       if g["state_bits"] not in (8, 32):
         raise ValueError("state_bits must be 8 or 32, got %r" % (g["state_bits"],))
       for p in g["params"]:
+        if not torch.is_tensor(p):
+          raise ValueError("parameters must be tensors, got %s" % type(p).__name__)
+        if not (p.is_leaf or p.retains_grad):
+          raise ValueError("a parameter is the result of an operation: it has no .grad to step from")
         if id(p) in seen:
           raise ValueError("a parameter appears more than once")
         seen.add(id(p))

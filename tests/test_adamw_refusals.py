@@ -107,3 +107,24 @@ def test_zero_grad_in_place():
   opt.zero_grad(set_to_none=False)
   assert flat.tolist() == [1.0] * 2 + [0.0] * 5 + [1.0] * 3 and p.grad.data_ptr() == flat[2:].data_ptr()
   assert all((t.grad == 0).all() and not t.grad.requires_grad for t in (p, q, r))
+
+
+def test_what_is_no_list_of_leaves():
+  """A tensor in place of a list (whose rows would be stepped without gradients, that is not at all), results of operations,
+  names beside parameters."""
+  from oi_vae_amd import optim
+  w = torch.zeros(3, 4, requires_grad=True)
+  for cls in (optim.AdamW, optim.Adam, optim.SGD):
+    with pytest.raises(TypeError, match="one tensor"):
+      cls(w)
+    group = cls([{"params": w}]).param_groups[0]
+    assert len(group["params"]) == 1 and group["params"][0] is w
+  for bad in ([w * 2], [w[0]], [{"params": [w, w.t()]}]):
+    with pytest.raises(ValueError, match="result of an operation"):
+      optim.AdamW(bad)
+  for bad in ([("w", w)], {"params": [w]}, [{"params": "w"}]):
+    with pytest.raises(ValueError, match="must be tensors"):
+      optim.AdamW(bad)
+  kept = w * 2
+  kept.retain_grad()
+  optim.AdamW([kept, w])
