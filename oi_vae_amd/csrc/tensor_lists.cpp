@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <algorithm>
+#include <utility>
 #include <vector>
 
 #include <ATen/core/Tensor.h>
@@ -115,8 +116,8 @@ PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 // gradients(list, records of oivae_grad_t, whether they will be written) -> (count, device, address of the
-// records) of the gradients that are there, or None when one is unusual,
-// appears twice or is on another device; (0, -1, address) without any.
+// records) of the gradients that are there, or None when one is unusual, shares memory with another (or appears twice) or is
+// on another device; (0, -1, address) without any.
 PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 3 || !PyList_Check(args[0])) {
     PyErr_SetString(PyExc_TypeError, "gradients(list, records, written)");
@@ -130,7 +131,7 @@ PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   long count = 0;
   int device = -1;
   try {
-    std::vector<void*> seen;
+    std::vector<std::pair<const char*, const char*>> seen;   // first byte, one past the last
     seen.reserve((size_t)n);
     for (Py_ssize_t i = 0; i < n; ++i) {
       PyObject* o = PyList_GET_ITEM(args[0], i);
@@ -140,10 +141,14 @@ PyObject* gradients(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (device < 0 && g.is_cuda()) device = (int)g.get_device();
       if (!plain(g, device)) Py_RETURN_NONE;
       r[count++] = oivae_grad_t{g.data_ptr(), g.numel(), type_of(g), -1};
-      if (g.numel() > 0) seen.push_back(g.data_ptr());
+      if (g.numel() > 0) {
+        const char* at = static_cast<const char*>(g.data_ptr());
+        seen.emplace_back(at, at + g.numel() * (type_of(g) == OIVAE_F32 ? 4 : 2));
+      }
     }
     std::sort(seen.begin(), seen.end());
-    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
+    for (size_t i = 1; i < seen.size(); ++i)
+      if (seen[i].first < seen[i - 1].second) Py_RETURN_NONE;
     for (Py_ssize_t i = 0; write && i < n; ++i) {
       const at::Tensor& g = THPVariable_Unpack(PyList_GET_ITEM(args[0], i)).grad();
       if (g.defined()) written(g);

@@ -186,6 +186,12 @@ def _grads_of(parameters, write):
   device = _check_types(grads, "gradients")
   if len({g.data_ptr() for g in grads if g.numel()}) != sum(1 for g in grads if g.numel()):
     raise ValueError("the same gradient appears more than once")
+  if write:   # what cannot be written is refused before the others are
+    if any(st == 0 and size > 1 for g in grads for st, size in zip(g.stride(), g.shape)):
+      raise RuntimeError("an expanded gradient (several elements in one place) cannot be scaled in place")
+    spans = sorted((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()) for g in grads if g.numel() and _dense(g))
+    if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+      raise ValueError("two gradients share memory")
   with torch.no_grad():
     packed = [g if _dense(g) else torch.empty(g.shape, dtype=g.dtype, device=device).copy_(g) for g in grads]
   rec = np.zeros(len(grads), _GRAD)

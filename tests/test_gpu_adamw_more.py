@@ -214,3 +214,30 @@ def test_a_limit_changed_between_steps():
   opt.max_grad_norm = None
   opt.step()
   assert opt.steps() == [4, 4]
+
+
+def test_clipping_refuses_what_it_cannot_scale_before_it_scales_anything():
+  """An expanded gradient, and gradients that share some memory, beside plain ones: nothing is written.  The norm alone reads them."""
+  from oi_vae_amd import optim
+  flat = torch.ones(100, device="cuda")
+  for grads, error in (([torch.ones(1, device="cuda").expand(50)], RuntimeError),
+                       ([torch.ones(1, 7, device="cuda").expand(5, 7)], RuntimeError),
+                       ([flat[:60], flat[59:]], ValueError), ([flat, flat[10:20]], ValueError),
+                       ([flat[:60], flat[10:20], flat[70:80]], ValueError)):
+    ps = [torch.zeros(g.shape, device="cuda").requires_grad_() for g in [torch.ones(40)] + grads]
+    for p, g in zip(ps, [torch.ones(40, device="cuda")] + grads):
+      p.grad = g
+    for order in (ps, ps[::-1]):
+      with pytest.raises(error):
+        optim.clip_grad_norm_(order, 1e-3)
+      assert all((p.grad == 1).all() for p in ps)
+      assert abs(optim.grad_norm(order).item() - np.sqrt(sum(p.numel() for p in ps))) <= 2.0 ** -23 * 20
+  ps = [torch.zeros(g.shape, device="cuda").requires_grad_() for g in (flat[:60], flat[60:])]      # neighbours share nothing
+  ps[0].grad, ps[1].grad = flat[:60], flat[60:]
+  optim.clip_grad_norm_(ps, 1.0)
+  assert ((flat - 0.1).abs() <= 2.0 ** -23).all()
+  wide = torch.ones(100, device="cuda")                                                            # interleaved: neither
+  q = [torch.zeros(50, device="cuda").requires_grad_() for _ in range(2)]
+  q[0].grad, q[1].grad = wide[::2], wide[1::2]
+  optim.clip_grad_norm_(q, 1.0)
+  assert ((wide - 0.1).abs() <= 2.0 ** -23).all()
