@@ -22,3 +22,34 @@ def test_flags_and_headers_rebuild_every_object(changed):
   for target in ("liboivae_hip.so", "liboivae_hip_waittest.so", "c_host_prox"):
     assert re.search(r"-o \S*/%s\s" % re.escape(target), out + "\n"), target
   assert changed.endswith("common.h") or re.search(r"-o \S*/_tensor_lists\.so\b", out)
+
+
+def _sources():
+  return [f for pattern in ("oi_vae_amd/csrc/*", "tools/probe/*.hip", "examples/*") for f in glob.glob(os.path.join(ROOT, pattern)) if f.endswith((".hip", ".h", ".cpp"))]
+
+
+def test_no_source_writes_packed_fp32_instructions():
+  """The flags keep the compiler from forming them; by hand they do not assemble under these flags either."""
+  assert len(_sources()) > 20
+  for f in _sources():
+    for line in open(f).read().split("\n"):
+      assert not re.search(r'"[^"]*v_pk_(add|mul|fma)_f32', line), (f, line)
+
+
+def test_loads_in_inline_assembly_wait_in_their_block():
+  """The compiler takes an asm block's outputs as written where the block ends."""
+  for f in _sources():
+    for block in re.findall(r"\basm\s*(?:volatile)?\s*\((.*?)\)\s*;", open(f).read(), re.S):
+      text = "".join(re.findall(r'"((?:[^"\\]|\\.)*)"', block))
+      if re.search(r"\b(global_load|flat_load|buffer_load|ds_read|ds_load|s_load)\w*", text) and " lds" not in text:
+        assert "s_waitcnt" in text, (f, block)
+
+
+@pytest.mark.parametrize("probe", ["mfma_probe2", "mfma_probe3"])
+def test_probes_build_with_the_documented_flags(probe, tmp_path):
+  """The two that held packed instructions."""
+  readme = open(os.path.join(ROOT, "tools", "probe", "README.md")).read()
+  flags = re.search(r"`hipcc (.*?) tools/probe/X\.hip", readme).group(1).split()
+  assert "-packed-fp32-ops" in flags and "--offload-arch=gfx950" in flags
+  subprocess.run(["/opt/rocm/bin/hipcc"] + flags + ["--cuda-device-only", "-c", "tools/probe/%s.hip" % probe, "-o", str(tmp_path / "probe.o")],
+                 check=True, cwd=ROOT, stderr=subprocess.DEVNULL)

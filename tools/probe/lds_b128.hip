@@ -32,12 +32,27 @@ __global__ __launch_bounds__(256) void k(const int* addr, int wr, int iters, uns
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     } else {
       u32x4 v[16];
-#pragma unroll
-      for (int u = 0; u < 16; ++u) {
-        if (u & 1) asm volatile("ds_read_b128 %0, %1 offset:32768" : "=v"(v[u]) : "v"(ba) : "memory");
-        else asm volatile("ds_read_b128 %0, %1" : "=v"(v[u]) : "v"(ba) : "memory");
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      // sixteen reads and their wait in one block: the registers are the compiler's only once they hold the data
+      asm volatile(
+          "ds_read_b128 %0, %16\n"
+          "ds_read_b128 %1, %16 offset:32768\n"
+          "ds_read_b128 %2, %16\n"
+          "ds_read_b128 %3, %16 offset:32768\n"
+          "ds_read_b128 %4, %16\n"
+          "ds_read_b128 %5, %16 offset:32768\n"
+          "ds_read_b128 %6, %16\n"
+          "ds_read_b128 %7, %16 offset:32768\n"
+          "ds_read_b128 %8, %16\n"
+          "ds_read_b128 %9, %16 offset:32768\n"
+          "ds_read_b128 %10, %16\n"
+          "ds_read_b128 %11, %16 offset:32768\n"
+          "ds_read_b128 %12, %16\n"
+          "ds_read_b128 %13, %16 offset:32768\n"
+          "ds_read_b128 %14, %16\n"
+          "ds_read_b128 %15, %16 offset:32768\n"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]), "=&v"(v[8]), "=&v"(v[9]), "=&v"(v[10]), "=&v"(v[11]), "=&v"(v[12]), "=&v"(v[13]), "=&v"(v[14]), "=&v"(v[15])
+          : "v"(ba) : "memory");
 #pragma unroll
       for (int u = 0; u < 16; ++u) s += v[u];
     }
