@@ -53,3 +53,13 @@ def test_probes_build_with_the_documented_flags(probe, tmp_path):
   assert "-packed-fp32-ops" in flags and "--offload-arch=gfx950" in flags
   subprocess.run(["/opt/rocm/bin/hipcc"] + flags + ["--cuda-device-only", "-c", "tools/probe/%s.hip" % probe, "-o", str(tmp_path / "probe.o")],
                  check=True, cwd=ROOT, stderr=subprocess.DEVNULL)
+
+
+def test_build_compiles_everything_every_time(monkeypatch):
+  import __graft_entry__ as entry
+  from oracle import prox_oracle
+  calls = []
+  monkeypatch.setattr(entry.subprocess, "check_call", lambda argv, **kw: calls.append(argv))
+  monkeypatch.setattr(prox_oracle, "build", lambda force=False: calls.append(force))
+  entry.build()
+  assert calls[0][0] == "make" and "-B" in calls[0] and calls[1:] == [True]
