@@ -262,7 +262,10 @@ __device__ __forceinline__ void conclude(const GradLaunch& a, const double* part
     oivae_step_t& q = v.steps[index - 1];
     const int t = q.t + 1;
     q.t = t;
-    // 1 - b^t = -expm1(t ln b) keeps its digits where b^t is near 1 (t = 1, b2 = 0.999)
+    // 1 - b^t = -expm1(t ln b) keeps its digits where b^t is near 1 (t = 1, b2 = 0.999).  In fp32 but for t ln b: within
+    // 4 * 2^-24 of the exact corrections, where the host rounds fp64 ones (run_adamw) -- a step that counts on the device may
+    // differ from one that counts on the host in the last places of step_size.  In fp64 the concluding block, which
+    // the step waits for, would take an exponential, a root and two quotients of many times the instructions
     q.inv_bc1 = 1.f / -expm1f((float)(t * v.ln_b1));
     q.inv_bc2_sqrt = 1.f / sqrtf(-expm1f((float)(t * v.ln_b2)));
   }
@@ -300,8 +303,10 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const double* __restrict
 }
 
 // g *= coef, one chunk a block.  With parts > 0 every block adds the partial sums itself, and the first one of the first launch
-// leaves the norm: cheaper than a launch between for few chunks (5.8M fp16, 800 chunks: norm and scaling 15.6 against 17.5 us),
-// dearer for many (67M bf16, 8264: 76.7 against 75.9; 268M fp32, 65600: 605 against 589).  HBM-bound: 268M fp32 gradients in 410 us behind the norm
+// leaves the norm: cheaper than a launch between for few chunks, the same or dearer for many.  Norm and scaling in us, every
+// block / a launch between, fp32: 256 chunks 9.9 / 13.0, 800 12.5 / 14.6, 1500 15.6 / 17.4, 2048 17.9 / 19.6, 3000 28.5 / 28.6,
+// 8264 80.7 / 80.6, 16384 152 / 149, 65600 605 / 589; bf16: 800 13.9 / 15.9, 2048 19.5 / 20.5, 3000 29.9 / 30.2, 16384 153 / 154.
+// HBM-bound: 268M fp32 gradients in 410 us behind the norm
 // (5.2 TB/s), 196 us with it when nothing has to be scaled.  One vector a thread scales them in 382 us, but then four times
 // the waves start only to read that the coefficient is one (237 us with the norm).
 __global__ __launch_bounds__(kThreads) void grad_clip_kernel(GradLaunch a, const double* __restrict__ part, int parts, float max_norm,
@@ -503,7 +508,7 @@ __device__ __forceinline__ float scale_of(uint32_t byte) {
 // 32 lanes hold one block, four elements each (one vector per thread and stream, as above).  With 16 lanes and 8 elements
 // a lane the vectors of a wave are 32 bytes apart: 861 us on 268M bf16 parameters against 719.
 //   kFast: hardware root and reciprocal (one unit in the last place each) instead of the correctly rounded ones, about a
-// third of the instructions: 719 against 779 us (694 now, 6.2 TB/s).  The hardware root takes subnormals for zero: up to
+// third of the instructions: 719 against 779 us (704 now, 6.1 TB/s).  The hardware root takes subnormals for zero: up to
 // 1.1e-19, times 1 / sqrt(1 - b2) at most, in a denominator of at least eps.
 template <bool kFast>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(AdamwLaunch a) {

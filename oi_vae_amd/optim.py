@@ -262,8 +262,13 @@ class AdamW(_EngineOptimizer):
   Handed to OIVAE, the norm is that of every gradient but Ws's, which SGD applies unclipped; a gradient of Ws that is not
   finite leaves the step out too (the norm is NaN then), and a step that is left out leaves Ws alone as well.
   capturable: keeps the step counts on the device, so that a step captured into a graph advances them (max_grad_norm
-  implies it); `lr` may then be a one-element float32 tensor on the device, which replays read anew.  Touch `buffers` (or
-  take a step) before capturing.  Nothing here synchronises."""
+  implies it); `lr` may then be a one-element float32 tensor on the device, which replays read anew.  Every other number --
+  weight_decay, grad_scale, max_grad_norm -- and the gradients' addresses are those of the capture.  Touch `buffers` (or
+  take a step) before capturing.  Counts on the device form their bias corrections there, in float32: such a step may differ
+  from one without `capturable` in its last places.  A step behind a failed decoder launch is left out on the device; counts on
+  the device stay then, counts on the host have moved when the host hears of it (at its next call, with an OivaeError).
+  Steps of one optimizer follow each other: they share its buffers.  It is no torch.optim.Optimizer: a schedule writes
+  `param_groups[k]["lr"]`.  Nothing here synchronises but `steps` and `state_dict` of counts on the device."""
 
   def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_grad_norm=None,
                capturable=False, seed=0):

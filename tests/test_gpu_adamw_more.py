@@ -241,3 +241,49 @@ def test_clipping_refuses_what_it_cannot_scale_before_it_scales_anything():
   q[0].grad, q[1].grad = wide[::2], wide[1::2]
   optim.clip_grad_norm_(q, 1.0)
   assert ((wide - 0.1).abs() <= 2.0 ** -23).all()
+
+
+def test_moments_of_8_bits_follow_the_exact_ones_over_many_steps():
+  """3000 steps of the kernel on Gaussian gradients whose scales spread over two decades in a block, against exact moments: the
+  codes' expectation is exact, so the mean over 8192 elements is too, up to six of its standard deviations.  Second moments:
+  0.53 of the moment an element (test_adamw_codes.py), 6 * 0.53 / sqrt(8192) = 0.036.  First moments, in units of the gradients'
+  sigma: a step moves m by (1 - b1) (g - m), 0.083 in the mean; a spacing is m / 8 at most, 0.023 in the mean (m's own sigma is
+  0.23), and 2^-16 of the block's largest, 0.003, for the smallest; 1 / (1 - b1^2) steps: a variance of at most 5.3 * 0.083 *
+  0.026 = 0.0114, 0.107 an element, 6 * 0.107 / sqrt(8192) = 0.0071."""
+  from oi_vae_amd import optim
+  n, b1, b2 = 8192, 0.9, 0.999
+  gen = torch.Generator(device="cuda").manual_seed(5)
+  sigma = 10 ** (-3 + 2 * torch.rand(n, generator=gen, device="cuda"))
+  p = torch.zeros(n, device="cuda").requires_grad_()
+  p.grad = torch.empty(n, device="cuda")
+  opt = optim.AdamW([p], lr=1e-4, betas=(b1, b2), state_bits=8)
+  m = v = torch.zeros(n, dtype=torch.float64, device="cuda")
+  for _ in range(3000):
+    torch.mul(sigma, torch.randn(n, generator=gen, device="cuda"), out=p.grad)
+    opt.step()
+    m = b1 * m + (1 - b1) * p.grad.double()
+    v = b2 * v + (1 - b2) * p.grad.double() ** 2
+  held = opt.buffers[8]
+  got = {k: held[k].double() * held[k + "_scale"].double().repeat_interleave(128) for k in ("exp_avg", "exp_avg_sq")}
+  assert abs((got["exp_avg_sq"] / v).mean().item() - 1.0) <= 0.036
+  assert abs(((got["exp_avg"] - m) / sigma).mean().item()) <= 0.0071
+  assert opt.steps() == [3000] and torch.isfinite(p).all()
+
+
+@pytest.mark.parametrize("b1,b2", [(0.9, 0.999), (0.9, 0.95), (0.0, 0.9999999), (0.999, 0.0)])
+def test_bias_corrections_on_the_device(b1, b2):
+  """1 / (1 - b1^t) and 1 / sqrt(1 - b2^t) of steps that count on the device, formed in float32 there: the exponent's rounding
+  (at most its own 2^-24 in 1 - b^t), the exponential's last place (2^-23) and the quotient's half make 4 * 2^-24, half of the
+  first two, the root's half and the quotient's 3.5 * 2^-24."""
+  from oi_vae_amd import optim
+  p = torch.ones(3, device="cuda").requires_grad_()
+  p.grad = torch.ones(3, device="cuda")
+  opt = optim.AdamW([p], lr=0.0, betas=(b1, b2), capturable=True)
+  u = 2.0 ** -24
+  for t in list(range(1, 20)) + [50, 100, 333, 1000, 4321, 10 ** 4, 10 ** 5, 10 ** 6, 2 * 10 ** 9]:
+    opt.set_steps(t - 1)
+    opt.step()
+    c1, c2 = opt._steps_dev[0].view(torch.float32)[1:3].double().tolist()
+    e1 = 1.0 if b1 == 0 else -np.expm1(t * np.log(b1))
+    e2 = 1.0 if b2 == 0 else -np.expm1(t * np.log(b2))
+    assert abs(c1 * e1 - 1.0) <= 4.01 * u and abs(c2 * np.sqrt(e2) - 1.0) <= 3.51 * u, (t, (c1 * e1 - 1) / u, (c2 * np.sqrt(e2) - 1) / u)
