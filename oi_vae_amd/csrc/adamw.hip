@@ -475,8 +475,9 @@ __global__ __launch_bounds__(kThreads) void adamw32_kernel(AdamwLaunch a) {
 //   The power of two brings the block's largest magnitude into [2^7, 2^8) (e4m3's largest is 448) or [2^14, 2^15) (57344),
 // so rounding up never leaves the format.  v_cvt_sr_fp8_f32 / v_cvt_sr_bf8_f32 add the upper 20 or 21 of 32 random bits
 // below the code's last place and cut off, subnormal codes included.
-constexpr uint32_t kMix1 = 0x9E3779B1u, kMix2 = 0x6A09E667u, kMix3 = 0xBB67AE85u, kMix4 = 0x3C6EF373u;   // 2^32 times the
-// fractions of the golden ratio and of the roots of 2, 3 and 5, made odd
+constexpr uint32_t kMix1 = 0x9E3779B1u, kMix2 = 0x6A09E667u, kMix3 = 0xBB67AE85u, kMix4 = 0x3C6EF373u;   // odd, with
+// no pattern in their bits: a prime near 2^32 times the golden ratio's fraction, and 2^32 times the fractions of the roots of
+// 2, 3 and 5
 
 __device__ __forceinline__ uint32_t random_key(uint32_t seed, uint32_t step, uint32_t tensor) {
   uint32_t k = seed * kMix1 + step * kMix3 + tensor * kMix4;
