@@ -139,12 +139,13 @@ def _check_types(tensors, what):
   return device
 
 
+_ZERO = 2.0 ** -150     # half of float32's smallest: what is not above it is zero there
+
+
 def _limit(max_norm, what="max_norm"):
-  """max_norm as a number, refused where float32, which the kernels compare in, has no positive value for it."""
-  number = float(max_norm)
-  if not number > 2.0 ** -150:     # half of float32's smallest
+  """Refuses a limit for which float32, in which the kernels compare, has no positive value."""
+  if not float(max_norm) > _ZERO:
     raise ValueError("%s must be positive (and not below float32's range), got %r" % (what, max_norm))
-  return number
 
 
 def _lists():
@@ -229,7 +230,9 @@ def grad_norm(parameters):
 def clip_grad_norm_(parameters, max_norm):
   """torch.nn.utils.clip_grad_norm_ (2-norm): scales the gradients in place by min(1, max_norm / (norm + 1e-6)) and returns
   the norm they had, without synchronising.  A norm that is not finite reaches the gradients as it does there (NaN)."""
-  max_norm = _limit(max_norm)
+  max_norm = float(max_norm)
+  if not max_norm > _ZERO:
+    _limit(max_norm)
   got = _grads_of(parameters, True)
   if got is None:
     return torch.zeros((), dtype=torch.float32)
@@ -607,7 +610,9 @@ class AdamW(_EngineOptimizer):
       groups[q] = self._lr_on_device(lr, g) if torch.is_tensor(lr) else (lr, g["weight_decay"], 0)
     limit = 0.0
     if self.max_grad_norm is not None:
-      limit = _limit(self.max_grad_norm, "max_grad_norm")
+      limit = float(self.max_grad_norm)
+      if not limit > _ZERO:
+        _limit(limit, "max_grad_norm")
       if not self._on_device:
         raise RuntimeError("max_grad_norm has to be given to the constructor (it may be changed or set to None later)")
     if not self._on_device and torch.cuda.is_current_stream_capturing():
