@@ -267,8 +267,7 @@ class AdamW(_EngineOptimizer):
   capturable: keeps the step counts on the device, so that a step captured into a graph advances them (max_grad_norm
   implies it); `lr` may then be a one-element float32 tensor on the device, which replays read anew.  Every other number --
   weight_decay, grad_scale, max_grad_norm -- and the gradients' addresses are those of the capture.  Touch `buffers` (or
-  take a step) before capturing.  Counts on the device form their bias corrections there, in float32: such a step may differ
-  from one without `capturable` in its last places.  A step behind a failed decoder launch is left out on the device; counts on
+  take a step) before capturing.  A step behind a failed decoder launch is left out on the device; counts on
   the device stay then, counts on the host have moved when the host hears of it (at its next call, with an OivaeError).
   Steps of one optimizer follow each other: they share its buffers.  It is no torch.optim.Optimizer: a schedule writes
   `param_groups[k]["lr"]`.  Nothing here synchronises but `steps` and `state_dict` of counts on the device."""
