@@ -38,19 +38,25 @@ DEC_SOURCES = ("oi_vae_amd/csrc/dec_x3_64s.h", "oi_vae_amd/csrc/mfma_decoder.hip
                "oi_vae_amd/csrc/x3_split.h")
 
 
+BUILD_FILE = os.path.join("oi_vae_amd", "csrc", "Makefile")
+
+
 def decoder_source_digest():
+  """Of the decoder's sources and of the flags that they are compiled with."""
   import hashlib
   h = hashlib.sha256()
   for f in DEC_SOURCES:
     with open(os.path.join(ROOT, f), "rb") as fh:
       h.update(fh.read())
+  with open(os.path.join(ROOT, BUILD_FILE)) as fh:
+    h.update(next(line for line in fh if line.startswith("COMMON :=")).encode())
   return h.hexdigest()[:16]
 
 
 def pmc_traffic():
   """HBM bytes per decoder launch from the committed rocprofv3 PMC passes (profiles/README.md names the commands).
   Counters cannot be read from inside this process, so this is a committed measurement -- valid for THIS tree only if
-  it was taken from the same decoder sources: tools/pmc_summarize.py stamps the file with a digest of them, and a
+  it was taken from the same decoder sources and flags: tools/pmc_summarize.py stamps the file with a digest of them, and a
   stamp that does not match the tree's gives null (a stale figure is worse than none)."""
   try:
     d = json.load(open(os.path.join(ROOT, PMC_FILE)))

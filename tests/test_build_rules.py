@@ -63,3 +63,15 @@ def test_build_compiles_everything_every_time(monkeypatch):
   monkeypatch.setattr(prox_oracle, "build", lambda force=False: calls.append(force))
   entry.build()
   assert calls[0][0] == "make" and "-B" in calls[0] and calls[1:] == [True]
+
+
+def test_the_profile_stamp_covers_the_flags(tmp_path, monkeypatch):
+  """A decoder built with other flags is another decoder: its profile's stamp differs; other lines of the Makefile do not matter."""
+  import bench
+  was = bench.decoder_source_digest()
+  text = open(os.path.join(ROOT, bench.BUILD_FILE)).read()
+  for change, same in ((lambda s: s.replace("COMMON := -O3", "COMMON := -O2"), False), (lambda s: s + "# more\n", True)):
+    other = tmp_path / "Makefile"
+    other.write_text(change(text))
+    monkeypatch.setattr(bench, "BUILD_FILE", str(other))
+    assert (bench.decoder_source_digest() == was) == same
