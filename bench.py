@@ -1,13 +1,13 @@
 #!/usr/bin/env python3
 """bench.py -- oi-VAE train samples/s (fwd + bwd + optimizers + prox) on MI355X.
 
-Workload (BASELINE.json configs[3], "synthetic scale-up"): G=1024 groups x 64
+Workload ("synthetic scale-up"): G=1024 groups x 64
 dims, K=64, two-layer generators Linear(64,64)->Tanh->Linear(64,64), global
 batch 65536, S=1, synthetic X ~ U[0,1) resident in HBM, random-init weights.
 One step = encoder fwd + reparam + KL, grouped decoder fwd+bwd, encoder bwd,
 weight prior + penalty, [gradient all-reduce over RCCL when N>1], fused Adam,
 fused SGD + proximal step.  N>1: one process per GPU (torchrun), the global
-batch is sharded over ranks ("strong" scaling, as BASELINE.json states it).
+batch is sharded over ranks ("strong" scaling).
 
 Prints ONE JSON line on rank 0.
 """
@@ -26,7 +26,7 @@ if ROOT not in sys.path:
 G, DG, K, H, M = 1024, 64, 64, 64, 64
 GLOBAL_BATCH = 65536
 LR, WS_LR, LAM = 1e-3, 1e-4, 1.0
-FP32_MATRIX_PEAK_TFLOPS = 157.3  # MI355X_MICROARCH.md, chip-level parameters
+FP32_MATRIX_PEAK_TFLOPS = 157.3  # the chip's parameter table
 F16_MATRIX_PEAK_TFLOPS = 16 * 157.3  # dense fp16/bf16 MFMA = 16 x the fp32 matrix rate, same table (2516.8)
 # what the chip sustains on v_mfma_f32_16x16x32_f16 alone with random operands at its power limit
 # (tools/probe/mfma_shape_power.hip: 2006 TFLOP/s; the 32x32x16 shape reaches 1772-1852, all-zero operands 2445)
@@ -72,21 +72,21 @@ def pmc_traffic():
 
 
 def decoder_flops_per_row():
-  # ALGORITHMIC flops: fwd + dgrad + wgrad of the three per-group products (SURVEY.md section 8d)
+  # ALGORITHMIC flops: fwd + dgrad + wgrad of the three per-group products
   return 3 * G * (2 * K * H + 2 * H * M + 2 * M * DG)
 
 
 def decoder_executed_flops(rows):
   """fp32-equivalent flops the decoder kernels issue: Ws[g] and the generator's first Linear compose
   (no nonlinearity between them), so the row loop has 6 products of 2*64*64 flops per row
-  and group instead of 9, plus three 64^3 products per group outside it (DESIGN.md 3.1)."""
+  and group instead of 9, plus three 64^3 products per group outside it."""
   return rows * G * 6 * 2 * 64 * 64 + G * 3 * 2 * 64 ** 3
 
 
 def decoder_f16_flops(rows):
   """16-bit matrix flops dec_x3_64s issues in the row loop: each of the six fp32 products (64 x 32 x 64 per 32-row tile:
   eight 16 x 16 blocks, two reduction steps of 32) as three fp16 products: 288 v_mfma_f32_16x16x32_f16 of 2*16*16*32
-  flops per 32-row tile and group (DESIGN.md 3.0; dec_x3_64g issued the same flops as 144 32x32x16 instructions)."""
+  flops per 32-row tile and group (dec_x3_64g issued the same flops as 144 32x32x16 instructions)."""
   return (rows + 31) // 32 * G * 288 * (2 * 16 * 16 * 32)
 
 
@@ -117,7 +117,7 @@ def init_engine(device, batch_rows, seed):
 
 
 def prox_roofline(device):
-  """Secondary measurement (BASELINE.json configs[4], wide-prox stress): the fused
+  """Secondary measurement (wide-prox stress): the fused
   SGD + proximal kernel on G=8192 x K=256 x H=8, threshold at the median row norm
   (about half of the rows die).  HBM-bound: 12 B/element (Ws read+write, dWs read)
   + 5 B/row (mask byte + norm)."""
@@ -406,7 +406,7 @@ def main():
                    "fp32_equivalent": {"executed_flops_per_launch": exe, "executed_tflops": tf(exe),
                                        "algorithmic_over_fp32_matrix_peak": tf(alg) / FP32_MATRIX_PEAK_TFLOPS,
                                        "fp32_matrix_peak": FP32_MATRIX_PEAK_TFLOPS},
-                   "note": "achieved/frac: the reference algorithm's flops (SURVEY 8d: 3 G (2KH + 2HM + 2M D_g) per row = "
+                   "note": "achieved/frac: the reference algorithm's flops (3 G (2KH + 2HM + 2M D_g) per row = "
                            "75.5 MFLOP, x rows per launch) over the launch time, against the dense fp16 matrix peak -- the "
                            "pipe the kernel runs on.  issued_*: the 16-bit matrix flops the kernel ISSUES (288 "
                            "v_mfma_f32_16x16x32_f16 per 32-row tile and group): each fp32 product costs three fp16 "
@@ -417,7 +417,7 @@ def main():
                            "ENTRY POINT timed with HIP events on its stream: dec_x3_64s plus ~0.06 ms of helpers (max|z|, "
                            "the image of z, the range guard and its gated second launch); profiles/ holds the "
                            "rocprofv3 kernel trace of the same command.  The kernel is not matrix-bound: the chain "
-                           "wave's dependent sequence and the dz float atomics (8.6 GB per launch) bound it, DESIGN 3.0"},
+                           "wave's dependent sequence and the dz float atomics (8.6 GB per launch) bound it"},
       "step_model_tflops": (decoder_flops_per_row() + encoder_flops_per_row()) * GLOBAL_BATCH / (ms * 1e-3) / 1e12 / world,
       "entry_ms": {k: sum(v) / len(v) for k, v in per_kernel.items()},
       "entry_ms_note": "three untimed steps behind the timed region, every entry point bracketed by HIP events; inside "

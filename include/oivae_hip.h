@@ -43,7 +43,7 @@ enum {
 enum {
   OIVAE_GEN_LINEAR = 0,       /* Linear(H, D_g)                bars_data_oivae.py:97, meg_oi_vae.py:178 */
   OIVAE_GEN_TANH_LINEAR = 1,  /* Tanh -> Linear(H, D_g)        mo_mo_mocap_oivae.py:203-207 */
-  OIVAE_GEN_MLP = 2           /* Linear(H,M) -> Tanh -> Linear(M, D_g)   (BASELINE.json "2-layer generators") */
+  OIVAE_GEN_MLP = 2           /* Linear(H,M) -> Tanh -> Linear(M, D_g)   (two-layer generators) */
 };
 
 /* Shapes of one model.  group_off is a DEVICE array of G+1 int32 prefix sums of
@@ -91,13 +91,13 @@ const char* oivae_version(void);
  * the fp16-term kernels the workspace carries max|X| of the last pass over X from call to call; a kernel that
  * scales X by it records the maximum it reads itself and is repeated (a gated second launch) when the two powers
  * of two differ, so a stale, zeroed or foreign workspace costs one more pass of that kernel, never a wrong result
- * (DESIGN.md 3.0, tests/test_gpu_ranges.py).  Passing the same workspace every step avoids the repeats.
+ * (tests/test_gpu_ranges.py).  Passing the same workspace every step avoids the repeats.
  * A bounded wait inside the decoder kernels that runs out raises two error words, one host-visible and one on the
  * device.  Calls are asynchronous, so the host learns of it at the first entry point it calls AFTER the kernel has
  * run -- every entry point looks, and that call returns OIVAE_E_HIP -- which may be several calls later when the
- * host runs ahead.  The parameters are protected regardless: oivae_adam_f32, oivae_sgd_prox_f32 and oivae_prox_f32
- * read the device word on the device and leave their arguments untouched while it is raised, so the gradients of a
- * failed decoder launch are never applied.  oivae_check_errors (below) gives the definite answer for everything
+ * host runs ahead.  The parameters are protected regardless: oivae_adam_f32, oivae_adamw_*, oivae_sgd_prox_f32 (and
+ * _clip_f32) and oivae_prox_f32 read the device word on the device and leave their arguments untouched while it is
+ * raised, so the gradients of a failed decoder launch are never applied.  oivae_check_errors (below) gives the definite answer for everything
  * queued so far, e.g. behind the last step of a run. */
 int64_t oivae_workspace_bytes(const oivae_shape_t* shape, int64_t B, int32_t S);
 

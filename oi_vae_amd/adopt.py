@@ -1,8 +1,8 @@
 """Recognise a model built with the reference's API and move it into an Engine.
 
 The reference lets callers compose arbitrary torch modules; its scripts only
-ever build three generator shapes and one encoder shape (SURVEY.md section 8a,
-rows E and D).  `adopt` pattern-matches exactly those, reads the constants of the
+ever build three generator shapes and one encoder shape.
+`adopt` pattern-matches exactly those, reads the constants of the
 opaque lambda heads by probing them in float64, and re-points every parameter
 tensor at a view of the engine's flat device buffers.  Anything else is refused
 with a clear error: the engine hard-codes its heads, it does not trace Python.

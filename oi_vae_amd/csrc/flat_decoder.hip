@@ -36,7 +36,7 @@ bool flat_decoder_applies(const oivae_shape_t& s, int64_t N) {
   return N * gh * 4 <= ((int64_t)1 << 30);  // Hc fits 1 GiB of workspace
 }
 
-// The three products on two fp16 terms (round 2, last part): they have the encoder GEMMs' shapes -- a long-reduction
+// The three products on two fp16 terms: they have the encoder GEMMs' shapes -- a long-reduction
 // "NT" product (dz: N x K over G*H, = the encoder forward with X := dH, W := Wk), a weight-gradient "TN" product
 // (Ct: K x G*H over N, = the encoder backward with dpre := z) and Hc = z Wc^T (the forward kernel again, with the
 // latent dimension as its short reduction and the G*H columns as its 128-wide column tiles) -- so they run on

@@ -12,7 +12,7 @@
 // (per thread, per workgroup, then one workgroup over the partials): reproducible, and within fp32 rounding of the
 // reference's fp32 pairwise sum.
 //
-// Scope (DESIGN.md 7): the reference's training step cannot run with Gamma members -- _DistributionCat.logprob needs
+// Scope: the reference's training step cannot run with Gamma members -- _DistributionCat.logprob needs
 // `size`, which the reference's Gamma lacks (lib/distributions.py:82) -- so this is the evaluation-side operator,
 // reached from oi_vae_amd.distributions.Gamma.logprob on device tensors, not an epilogue of the fused step.
 #include "common.h"

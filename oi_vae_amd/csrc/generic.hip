@@ -1,7 +1,7 @@
 // Shape-generic kernels of the oi-VAE step (any K, H, M, ragged group dims).
 //
 // These are the correctness-first paths that serve the small, launch-bound
-// configurations (bars, mocap, MEG: SURVEY.md section 8 C1-C3, C5) and every shape
+// configurations (bars, mocap, MEG) and every shape
 // the MFMA fast paths (mfma_*.hip) do not cover.  All reductions that feed
 // parameter gradients run in a fixed order (per-block slabs, summed in index
 // order), so decoder and encoder weight gradients are reproducible run to run;
@@ -641,7 +641,7 @@ __global__ __launch_bounds__(256) void enc_bwd_pre(int64_t B, int K, int S, cons
   if (dz_sn == 1 && S == 1) {
     // dz arrives transposed ([K, N], the matrix-core decoders): consecutive threads of the element loop below meet
     // consecutive k, i.e. addresses N floats apart.  Tiles of 64 rows are therefore read along n (256-byte runs) into
-    // LDS first (round 2: 84 -> 25 us at 65536 rows).
+    // LDS first (84 -> 25 us at 65536 rows).
     float* sT = reinterpret_cast<float*>(col + 2 * K + 512);   // [K][65]
     for (int64_t t0 = r0; t0 < r1; t0 += 64) {
       const int nr = (int)((r1 - t0 < 64) ? r1 - t0 : 64);

@@ -617,7 +617,7 @@ int launch_decoder_mfma(const oivae_shape_t& s, const oivae_tensors_t* params, c
   // test hooks: OIVAE_DEC=v1 the layer-by-layer fp32 template kernel (which also serves launches whose dz image
   // exceeds the 32-bit byte offsets of dec_mfma64_v4's atomics, N*K*4 >= 2^32), OIVAE_DEC=v4 the fp32
   // composed-first-layer kernel, OIVAE_DEC=x3 the single-wave-per-SIMD split-bf16 kernel, OIVAE_DEC=p the all-bf16
-  // pair of waves, OIVAE_DEC=g dec_x3_64g (32x32x16 fp16 instructions; round 2's default until dec_x3_64s), OIVAE_DEC=s
+  // pair of waves, OIVAE_DEC=g dec_x3_64g (32x32x16 fp16 instructions; the default before dec_x3_64s), OIVAE_DEC=s
   // (= unset) dec_x3_64s, the default below
   const bool force_v1 = dec_env != nullptr && dec_env[0] == 'v' && dec_env[1] == '1';
   const bool use_x3 = (dec_env != nullptr && (dec_env[0] == 'x' || dec_env[0] == 'p')) ||

@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256, (ND == 1 ? 2 : 1)) void enc_bwd_gemm(const flo
     // Operands of k-step s+1 are read from LDS before the MFMAs of k-step s (two register sets), so the matrix
     // pipe never waits for an LDS round trip inside a tile.  Volatile LDS pointers keep the reads in this order
     // and out of ds_read2_b32 (whose 8-bit offsets would cost a VALU add per pair; a VALU instruction costs ~8
-    // cycles of fp32 matrix time, an LDS read ~1-2: DESIGN.md 3.1).
+    // cycles of fp32 matrix time, an LDS read ~1-2).
     const ldsv_t p = (ldsv_t)(sP + (t & 1) * 32 * BJ + hh * BJ + l31);
     const ldsv_t x = (ldsv_t)(sX + (t & 1) * 32 * BD + hh * BD + wave * (32 * ND) + l31);
     float fa[2][TJ], fb[2][ND];

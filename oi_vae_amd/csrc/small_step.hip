@@ -1,7 +1,7 @@
 // The whole training step of a SMALL oi-VAE in one launch: the shapes the reference's own scripts train
 // (bars_data_oivae.py: 8 groups of 8 pixels, K = 8..16, H = 1, batch 64; mo_mo_mocap_oivae.py: 29 joints of 1..3
 // angles, K = 8, H = 8, batch 64 x 10 samples).  At these sizes the step of the large-model kernels is two dozen
-// launches of 4..8 us each -- launch-bound at 0.11 ms (DESIGN.md 3.5); here it is one memset node and one kernel:
+// launches of 4..8 us each -- launch-bound at 0.11 ms; here it is one memset node and one kernel:
 //
 //   every workgroup takes RB batch rows (with their S samples: NR = RB S decoder rows) through
 //     encoder forward + reparameterisation + KL            lib/models.py:15-16, lib/utils.py:9-18, lib/oivae.py:50-53
@@ -47,8 +47,8 @@ SmallPlan plan_small_step(const oivae_shape_t& s, int64_t B, int32_t S) {
   // few, fat workgroups: the step is latency-bound (a handful of dependent phases), and the last workgroup adds one
   // slab per workgroup -- about 30 decoder rows each, one (row, group) item per thread in the decoder phase
   const int64_t N = B * (int64_t)S;
-  // (rows per workgroup tried, us per step -- round 2: 24 / 48 / 96 / 192 rows: bars 35 / 34 / 40 / 44, mocap 61 / 59 / 79 / 99;
-  // round 3, outputs indexed by kind and loads batched: 24 / 30 / 40 / 48: bars 30.5 / 30.5 / 31.1 / 31.9, mocap 46.3 / 46.3 /
+  // (rows per workgroup tried, us per step: 24 / 48 / 96 / 192 rows: bars 35 / 34 / 40 / 44, mocap 61 / 59 / 79 / 99;
+  // with outputs indexed by kind and loads batched: 24 / 30 / 40 / 48: bars 30.5 / 30.5 / 31.1 / 31.9, mocap 46.3 / 46.3 /
   // 46.4 / 48.4: at 30 mocap's 29 groups are one decoder round)
   int nb = (int)((N + 29) / 30);
   if (nb > kSmallMaxBlocks) nb = kSmallMaxBlocks;   // larger batches: fatter workgroups, as far as LDS goes (checked below)

@@ -13,7 +13,7 @@
 // The three dropped ones (mid*lo, lo*mid, lo*lo) are below 2^-24 |a b|, i.e. below
 // the rounding of the fp32 product itself; each partial product of two bf16 numbers
 // is exact in fp32 and the matrix unit accumulates in fp32, so the result carries the
-// same error as the fp32 MFMA chain (measured: tests/test_gpu_scale.py, DESIGN.md 3.2).
+// same error as the fp32 MFMA chain (measured: tests/test_gpu_scale.py).
 // Non-finite inputs give NaN where the fp32 kernels give +-inf (inf - inf in the split).
 //
 // The streamed operand (X, 17 GB) is split in registers on its way into LDS; the small
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(768, 1) void enc_x3_gemm(const float* __restrict__ 
 // ------------------------------------------------------------------------------
 // Backward GEMM on two fp16 terms per operand ("h2", x3_split.h): [dWmu; dWsig] = dpre^T * X with THREE fp16 matrix
 // products per fp32 product instead of six bf16 ones -- half the matrix energy on a chip that runs these kernels at
-// its power limit (DESIGN.md 3.0).  fp16 has no exponent range to spare, so both operands are scaled by powers of two
+// its power limit.  fp16 has no exponent range to spare, so both operands are scaled by powers of two
 // taken from their true maxima: max|X| was recorded by the forward kernel's producers while they streamed the same X
 // (rng[0]), max|dpre| by absmax_f32 below (rng[2]); the result is scaled back in the epilogue.  Same tile, roles and
 // barrier schedule as enc_x3_gemm<true>; LDS rows are 20 dwords (2 pieces x 8 + 4 pad: conflict-free 16-byte reads).

@@ -3,11 +3,10 @@
 //   dec_x3_64      OIVAE_DEC=x3   three bf16 terms per operand (six products), one wave per SIMD
 //   dec_x3_64p     OIVAE_DEC=p    the same arithmetic, chain wave + weight-gradient wave per SIMD; also what a launch
 //                                 falls back to when dz exceeds 32-bit byte offsets or the parameters are unaligned
-//   dec_x3_64g     OIVAE_DEC=g    two fp16 terms, 32x32x16 instructions, two groups per workgroup (round 2's default
-//                                 until dec_x3_64s moved it to 16x16x32 instructions)
+//   dec_x3_64g     OIVAE_DEC=g    two fp16 terms, 32x32x16 instructions, two groups per workgroup (the default
+//                                 before dec_x3_64s moved it to 16x16x32 instructions)
 // Same mathematics as dec_x3_64s on other instructions and operand widths: the parity tests run several of them
-// against the oracle and against each other (tests/test_gpu_parity.py, test_gpu_x3.py, test_gpu_scale.py).  Their
-// design notes and measurements: HISTORY.md 3.0.
+// against the oracle and against each other (tests/test_gpu_parity.py, test_gpu_x3.py, test_gpu_scale.py).
 #include "dec_shared.h"
 
 namespace oivae {
@@ -1019,7 +1018,7 @@ __global__ __launch_bounds__(512, 1) void dec_x3_64p(MfmaDecArgs a) {
 
 // ------------------------------------------------------------------------------------------------------------
 // dec_x3_64g: dec_x3_64p on two fp16 terms per operand, with TWO groups per workgroup so that the sum over groups of
-// dz starts on chip.  (Its one-group predecessor dec_x3_64h, round 1's default, is gone: git history)
+// dz starts on chip.  (Its one-group predecessor dec_x3_64h is gone.)
 // fp16 terms: every chain operand is scaled by a power of two taken from its maximum -- the weight images from
 // reductions at set-up, z from a reduction before its image is built (rng[5]), t by 2^13 -- or from a bound of it:
 // |mu - x| <= max_d(|b2| + sum_m |W2|) + max|X| (rng[0]), |gmu| <= max c3 times that, |da1| <= max_m sum_d |W2| times

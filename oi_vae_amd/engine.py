@@ -1,8 +1,7 @@
 """Device-resident state and kernel sequencing of one oi-VAE on one MI355X.
 
 The engine owns two flat fp32 device buffers, parameters and gradients, laid
-out in the order the data-parallel gradient bucket uses
-(SURVEY.md section 8e):
+out in the order the data-parallel gradient bucket uses:
 
     [enc_Wmu | enc_bmu | enc_Wsig | enc_bsig | gen_W1 | gen_b1 | gen_W2 | gen_b2 | log_sigma | Ws]
 
@@ -30,7 +29,7 @@ _ALIGN = 64  # floats (256 B): keeps every segment 16-byte aligned for vector ac
 
 
 class ModelSpec:
-  """Shapes of one oi-VAE (names follow SURVEY.md section 8)."""
+  """Shapes of one oi-VAE: D outputs, K latent dimensions, G groups, H inputs of a group, M hidden units."""
 
   def __init__(self, D, K, H, group_dims, gen_type, M=0):
     self.D, self.K, self.H, self.M = int(D), int(K), int(H), int(M)

@@ -50,7 +50,7 @@ class Experiment(object):
         mu_net = torch.nn.Linear(group_input_dim, out_dim)
       elif gen_type == "tanh_linear":     # mo_mo_mocap_oivae.py:203-207
         mu_net = torch.nn.Sequential(torch.nn.Tanh(), torch.nn.Linear(group_input_dim, out_dim))
-      elif gen_type == "mlp":             # BASELINE.json "2-layer generators"
+      elif gen_type == "mlp":             # two-layer generators
         mu_net = torch.nn.Sequential(torch.nn.Linear(group_input_dim, hidden), torch.nn.Tanh(),
                                      torch.nn.Linear(hidden, out_dim))
       else:

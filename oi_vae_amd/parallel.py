@@ -1,7 +1,7 @@
 """Data-parallel glue: one process per GPU, torch.distributed over RCCL.
 
-The reference has no distributed code; the semantics are derived in SURVEY.md
-section 8e.  Every loss term except the weight prior is a sum divided by the
+The reference has no distributed code; the semantics follow from its loss.
+Every loss term except the weight prior is a sum divided by the
 local batch size (/root/reference/lib/oivae.py:50,55-59) and the weight prior is
 batch independent, so with equal shards the exact global-batch gradient is the
 MEAN over ranks of the local gradients.  One all-reduce over the engine's flat
@@ -52,7 +52,7 @@ class BucketedGradSync:
   all-reduce (60 % of the bytes at the scale-up shape) is issued right after it and
   runs on the communicator's stream while the encoder backward GEMM computes; the
   encoder part follows.  `wait()` makes the compute stream wait for both and must
-  be called before the optimizers and the proximal step (SURVEY.md section 8e);
+  be called before the optimizers and the proximal step;
   `wait_decoder()` / `wait_encoder()` wait for one bucket each, so that the decoder-side
   optimizers run under the encoder bucket's all-reduce (bench.py).
   Collectives are issued in the same order on every rank.  `holder` is anything

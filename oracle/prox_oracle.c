@@ -165,8 +165,8 @@ int oivae_oracle_prox_f32(float* Ws, long rows, int H, float t, const uint16_t* 
  * ------------------------------------------------------------------------- */
 static float multi_row_sumsq(const float* w, long stride, int n) {
   /* aten multi_row_sum, level step 16 for n < 2^20: level 0 is flushed into level 1 every 16 terms, level 1 into
-   * level 2 every 256, level 2 into level 3 every 4096.  (Until round 2's last part this kept two levels only, which
-   * is the same sum below 272 terms -- the recorded vectors went to 255 -- and a different one from there on.) */
+   * level 2 every 256, level 2 into level 3 every 4096.  (Two levels only are
+   * the same sum below 272 terms -- the first recorded vectors went to 255 -- and a different one from there on.) */
   float a[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   int i = 0;
   while (i + 16 <= n) {

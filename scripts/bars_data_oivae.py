@@ -18,7 +18,7 @@ from oi_vae_amd.experiments import Experiment  # noqa: E402
 def main(argv=None):
   ap = argparse.ArgumentParser()
   ap.add_argument("--iterations", type=int, default=20000)      # num_epochs, bars_data_oivae.py:30
-  ap.add_argument("--dim-z", type=int, default=8)               # image_size in the script; BASELINE.json runs 16 too
+  ap.add_argument("--dim-z", type=int, default=8)               # image_size in the script; 16 is run too
   ap.add_argument("--lam", type=float, default=1.0)
   ap.add_argument("--log-every", type=int, default=500)
   ap.add_argument("--torch-optimizers", action="store_true", help="caller-owned torch.optim instead of the fused kernels")

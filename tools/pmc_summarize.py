@@ -5,7 +5,7 @@ usage: pmc_summarize.py OUT.json DIR [DIR ...]
 
 Every DIR is the -d output directory of one `rocprofv3 --pmc ... --output-format csv`
 pass (tools/pmc_collect.sh).  Counters are averaged over the launches of each kernel
-of the `oivae::` namespace.  HBM bytes follow MI355X_MICROARCH.md section HBM:
+of the `oivae::` namespace.  HBM bytes:
 FETCH_SIZE is in KiB and reports half of the bytes of wide coalesced reads on
 gfx950 (so x1024 x2); WRITE_SIZE x1024 is exact for 16-byte stores and float atomics.
 """
