@@ -266,7 +266,7 @@ class AdamW(_EngineOptimizer):
   finite leaves the step out too (the norm is NaN then), and a step that is left out leaves Ws alone as well.
   capturable: keeps the step counts on the device, so that a step captured into a graph advances them (max_grad_norm
   implies it); `lr` may then be a one-element float32 tensor on the device, which replays read anew.  Every other number --
-  weight_decay, grad_scale, max_grad_norm -- and the gradients' addresses are those of the capture.  Touch `buffers` (or
+  weight_decay, grad_scale, max_grad_norm, seed -- and the gradients' addresses are those of the capture.  Touch `buffers` (or
   take a step) before capturing.  A step behind a failed decoder launch is left out on the device; counts on
   the device stay then, counts on the host have moved when the host hears of it (at its next call, with an OivaeError).
   Steps of one optimizer follow each other: they share its buffers.  It is no torch.optim.Optimizer: a schedule writes
@@ -389,7 +389,7 @@ class AdamW(_EngineOptimizer):
         k.grads = self._norm_rec[at:at + len(k.mine)]
         at += len(k.mine)
     self._buffers = buffers
-    self.sync_master()
+    self._take_master()
 
   @property
   def buffers(self):
@@ -415,6 +415,10 @@ class AdamW(_EngineOptimizer):
     for k in self._kinds:
       for p, r in zip(k.leaves, k.rec):
         self._check_parameter(p, r)
+    self._take_master()
+
+  @torch.no_grad()
+  def _take_master(self):
     for p, flat in self._views("master"):
       flat.as_strided(p.shape, p.stride()).copy_(p)
 
