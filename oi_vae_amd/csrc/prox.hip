@@ -20,9 +20,11 @@ namespace oivae {
 
 // Whether the step that this launch belongs to changes nothing: a decoder launch of it failed (common.h ErrWords), or the
 // verdict on its gradients (oivae_grad_norm) leaves it out -- the whole step, Ws among the rest: one step with a NaN in its
-// gradients would otherwise reach Ws, and through it every gradient of every later step.
-__device__ __forceinline__ bool left_out(const uint16_t* __restrict__ tab, const oivae_clip_t* __restrict__ clip) {
-  return *reinterpret_cast<const uint32_t*>(tab + kBadWordOffsetU16) != 0 || (clip != nullptr && clip->skip != 0);
+// gradients would otherwise reach Ws, and through it every gradient of every later step.  Without a verdict `skip` is the error
+// word again (launch_prox): two loads in flight together instead of a test of the pointer between them, which cost the
+// wide-prox launch 0.5 of its 36 us.
+__device__ __forceinline__ bool left_out(const uint16_t* __restrict__ tab, const int32_t* __restrict__ skip) {
+  return (*reinterpret_cast<const uint32_t*>(tab + kBadWordOffsetU16) | (uint32_t)*skip) != 0;
 }
 
 // ---- path A: any H, one thread per row, scalar emulation of the sum order ----
@@ -34,8 +36,8 @@ __global__ __launch_bounds__(256) void prox_rows_scalar(float* __restrict__ Ws,
                                                         uint8_t* __restrict__ mask,
                                                         float* __restrict__ norms,
                                                         const uint16_t* __restrict__ tab,
-                                                        const oivae_clip_t* __restrict__ clip) {
-  if (left_out(tab, clip)) return;
+                                                        const int32_t* __restrict__ skip) {
+  if (left_out(tab, skip)) return;
   const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (r >= rows) return;
   prox_row_scalar_dev<SGD>(Ws, dWs, r, H, neg_lr, t, do_prox, mask, norms, tab);
@@ -110,8 +112,8 @@ __global__ __launch_bounds__(256) void prox_rows_vec(float* __restrict__ Ws,
                                                      uint8_t* __restrict__ mask,
                                                      float* __restrict__ norms,
                                                      const uint16_t* __restrict__ tab,
-                                                     const oivae_clip_t* __restrict__ clip) {
-  if (left_out(tab, clip)) return;
+                                                     const int32_t* __restrict__ skip) {
+  if (left_out(tab, skip)) return;
   constexpr int H = 8 * V;
   const int64_t gt = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t r = gt >> 1;
@@ -161,8 +163,8 @@ __global__ __launch_bounds__(kProxLdsThreads, 1) void prox_rows_vec_lds(float* _
                                                                         uint8_t* __restrict__ mask,
                                                                         float* __restrict__ norms,
                                                                         const uint16_t* __restrict__ tab,
-                                                                        const oivae_clip_t* __restrict__ clip) {
-  if (left_out(tab, clip)) return;
+                                                                        const int32_t* __restrict__ skip) {
+  if (left_out(tab, skip)) return;
   constexpr int H = 8 * V;
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   uint16_t* ltab = reinterpret_cast<uint16_t*>(smem_raw);   // [65536]
@@ -225,8 +227,8 @@ __global__ __launch_bounds__(256) void prox_rows_wide(float* __restrict__ Ws, co
                                                       int64_t rows, int H, float neg_lr, float t, int do_prox,
                                                       uint8_t* __restrict__ mask, float* __restrict__ norms,
                                                       const uint16_t* __restrict__ tab,
-                                                      const oivae_clip_t* __restrict__ clip) {
-  if (left_out(tab, clip)) return;
+                                                      const int32_t* __restrict__ skip) {
+  if (left_out(tab, skip)) return;
   const int sub = threadIdx.x & 31;                                    // chain: accumulator k = sub / 8, lane l = sub % 8
   const int64_t r = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const bool live = r < rows;                                           // uniform per group of 32
@@ -375,7 +377,7 @@ __global__ __launch_bounds__(256) void prox_cols(float* __restrict__ W, const in
 
 template <int VV, bool SGD>
 static int launch_prox_vec(float* Ws, const float* dWs, int64_t rows, float neg_lr, float t, int do_prox, uint8_t* mask,
-                           float* norms, const uint16_t* tab, const oivae_clip_t* clip, hipStream_t st) {
+                           float* norms, const uint16_t* tab, const int32_t* skip, hipStream_t st) {
   // path C from 4 passes of 256 workgroups up (512 rows each per pass), for rows of at most 128 bytes (two rows per
   // thread in registers under 1024 threads per workgroup; at 256 bytes the fused-SGD form spills)
   if constexpr (VV <= 4) {
@@ -383,13 +385,13 @@ static int launch_prox_vec(float* Ws, const float* dWs, int64_t rows, float neg_
       OIVAE_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(&prox_rows_vec_lds<VV, SGD>),
                                           hipFuncAttributeMaxDynamicSharedMemorySize, 131072));
       hipLaunchKernelGGL((prox_rows_vec_lds<VV, SGD>), dim3(256), dim3(kProxLdsThreads), 131072, st, Ws, dWs, rows,
-                         neg_lr, t, do_prox, mask, norms, tab, clip);
+                         neg_lr, t, do_prox, mask, norms, tab, skip);
       return OIVAE_OK;
     }
   }
   const unsigned blocks = (unsigned)((rows * 2 + 255) / 256);
   hipLaunchKernelGGL((prox_rows_vec<VV, SGD>), dim3(blocks), dim3(256), 0, st, Ws, dWs, rows, neg_lr, t, do_prox, mask,
-                     norms, tab, clip);
+                     norms, tab, skip);
   return OIVAE_OK;
 }
 
@@ -399,11 +401,12 @@ static int launch_prox(float* Ws, const float* dWs, int64_t rows, int H, float l
   const uint16_t* tab = rsqrt14_table_device();
   if (!tab) return fail(OIVAE_E_NOINIT, "oivae_init has not been called on this device");
   if (rows == 0) return OIVAE_OK;
+  const int32_t* skip = clip ? &clip->skip : reinterpret_cast<const int32_t*>(tab + kBadWordOffsetU16);
   const float neg_lr = -lr;
   const bool aligned = ((reinterpret_cast<uintptr_t>(Ws) & 15) == 0) &&
                        (!SGD || (reinterpret_cast<uintptr_t>(dWs) & 15) == 0);
 #define OIVAE_PROX_VEC(VV)                                                                        \
-  { if (int rc = launch_prox_vec<VV, SGD>(Ws, dWs, rows, neg_lr, t, do_prox, mask, norms, tab, clip, st)) return rc; }
+  { if (int rc = launch_prox_vec<VV, SGD>(Ws, dWs, rows, neg_lr, t, do_prox, mask, norms, tab, skip, st)) return rc; }
   if (aligned && H == 8) OIVAE_PROX_VEC(1)
   else if (aligned && H == 16) OIVAE_PROX_VEC(2)
   else if (aligned && H == 32) OIVAE_PROX_VEC(4)
@@ -412,11 +415,11 @@ static int launch_prox(float* Ws, const float* dWs, int64_t rows, int H, float l
   else if (H >= 512) {
     const unsigned blocks = (unsigned)((rows * 32 + 255) / 256);
     hipLaunchKernelGGL((prox_rows_wide<SGD>), dim3(blocks), dim3(256), 0, st, Ws, dWs, rows, H,
-                       neg_lr, t, do_prox, mask, norms, tab, clip);
+                       neg_lr, t, do_prox, mask, norms, tab, skip);
   } else {
     const unsigned blocks = (unsigned)((rows + 255) / 256);
     hipLaunchKernelGGL((prox_rows_scalar<SGD>), dim3(blocks), dim3(256), 0, st, Ws, dWs, rows, H,
-                       neg_lr, t, do_prox, mask, norms, tab, clip);
+                       neg_lr, t, do_prox, mask, norms, tab, skip);
   }
 #undef OIVAE_PROX_VEC
   OIVAE_LAUNCH_CHECK();
