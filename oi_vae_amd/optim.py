@@ -545,8 +545,9 @@ class AdamW(_EngineOptimizer):
     """A state's options, as numbers, once they are known to be ones that this optimizer's groups could have been given."""
     out = []
     for g, src in zip(self.param_groups, groups):
-      if set(src) != set(g) - {"params"}:
-        raise ValueError("a group of the state has the options %s, here it has %s" % (sorted(src), sorted(set(g) - {"params"})))
+      strange = set(src) - set(g) | {"lr", "betas", "eps", "weight_decay", "state_bits"} - set(src)
+      if strange:
+        raise ValueError("a group of the state has other options than here: %s" % ", ".join(sorted(strange)))
       for k, v in list(src.items()) + [(k, v) for k, v in g.items() if k != "params"]:
         if torch.is_tensor(v) and v.numel() != 1:
           raise ValueError("%s has %d values" % (k, v.numel()))

@@ -301,3 +301,18 @@ def test_counts_on_the_device_and_on_the_host_give_one_step(bits):
       opt.step()
       runs.append(_snapshot(opt, ps))
     assert all(torch.equal(a, b) for a, b in zip(*runs)), t
+
+
+def test_keys_that_a_schedule_added_to_the_groups():
+  """Where the state has them too they are taken over; where it has not, the ones here stay."""
+  opt, _ = _made([[A], [B]])
+  state = opt.state_dict()
+  for k, g in enumerate(opt.param_groups):
+    g["initial_lr"] = 0.5 + k
+  opt.load_state_dict(state)
+  assert [g["initial_lr"] for g in opt.param_groups] == [0.5, 1.5]
+  state = opt.state_dict()
+  for g in opt.param_groups:
+    g["initial_lr"] = 7.0
+  opt.load_state_dict(state)
+  assert [g["initial_lr"] for g in opt.param_groups] == [0.5, 1.5]
