@@ -65,8 +65,9 @@ struct Buffer {
 };
 
 // parameters(list, records of oivae_adamw_tensor_t, device, records of oivae_grad_t or None) -> (first unusual tensor or -1,
-// number without a gradient).  Fills p, g and g_type, g = 0 where a parameter has no gradient, and the gradients' records
-// (n = 0 and index -1 there).  The records' n, p_type and pad (the order of its elements) say what the parameters have to be.
+// number without a gradient).  Fills p, g and g_type, g = 0 where a parameter has no gradient (an address that nothing reads
+// where it has one without elements, whose own is 0), and the gradients' records (n = 0 and index -1 there).  The records' n,
+// p_type and pad (the order of its elements) say what the parameters have to be.
 PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != 4 || !PyList_Check(args[0])) {
     PyErr_SetString(PyExc_TypeError, "parameters(list, records, device, gradient records)");
@@ -103,7 +104,7 @@ PyObject* parameters(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if ((rows ? 0 : order_of(p)) != r[i].pad) break;
       written(p);
       r[i].p = p.data_ptr();
-      r[i].g = g.data_ptr();
+      r[i].g = g.numel() > 0 ? g.data_ptr() : reinterpret_cast<void*>(16);
       r[i].g_type = type_of(g);
       if (q) q[i] = oivae_grad_t{g.data_ptr(), g.numel(), type_of(g), r[i].index};
       unusual = -1;

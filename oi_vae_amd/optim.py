@@ -585,7 +585,7 @@ class AdamW(_EngineOptimizer):
         g = torch.empty_like(p, dtype=g.dtype).copy_(g)
         copies.append(g)
       _written(p)
-      r["p"], r["g"], r["g_type"] = p.data_ptr(), g.data_ptr(), _TYPES[g.dtype]
+      r["p"], r["g"], r["g_type"] = p.data_ptr(), g.data_ptr() or 16, _TYPES[g.dtype]     # (0: no gradient)
       if kind.grads is not None:
         kind.grads[j] = (g.data_ptr(), g.numel(), _TYPES[g.dtype], r["index"])
     return missing

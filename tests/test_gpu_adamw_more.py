@@ -316,3 +316,23 @@ def test_keys_that_a_schedule_added_to_the_groups():
     g["initial_lr"] = 7.0
   opt.load_state_dict(state)
   assert [g["initial_lr"] for g in opt.param_groups] == [0.5, 1.5]
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(capturable=True), dict(max_grad_norm=1.0)])
+@pytest.mark.parametrize("odd", [False, True])      # a gradient in another order sends the list the way round the native reader
+def test_parameters_without_elements_count_their_steps(odd, kw):
+  from oi_vae_amd import optim
+  ps = _params([0, 5, 3], torch.float32, seed=1) + [torch.zeros(0, 4, device="cuda", requires_grad=True)]
+  ps[3].grad = torch.zeros(0, 4, device="cuda")
+  if odd:
+    ps.append(torch.zeros(6, 7, device="cuda", requires_grad=True))
+    ps[4].grad = torch.ones(7, 6, device="cuda").t()
+  opt = optim.AdamW(ps, lr=1e-2, **kw)
+  opt.step()
+  ps[1].grad = None
+  opt.step()
+  assert opt.steps() == [2, 1, 2, 2] + [2] * odd
+  for p in ps[2:3] + ps[4:]:
+    p.grad = None
+  opt.step()                    # those without elements alone
+  assert opt.steps() == [3, 1, 2, 3] + [2] * odd
